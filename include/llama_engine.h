@@ -105,8 +105,8 @@ const char* llama_tokenizer_decode(llama_tokenizer_t tokenizer, int32_t token_id
  * 8192).  Slot 0 is the sequence used by the Part-1 calls.  NULL on failure. */
 llama_engine_t llama_engine_create_ex(const char* model_path, int device, int max_batch, int max_seq_len);
 
-/* Message of the last failure on this handle (or of the last failed create when engine is
- * NULL).  Never NULL. */
+/* Message of the last failure on this handle (or, when engine is NULL, of the last failed create
+ * or the last refused llama_paged_* / llama_sample_rows call).  Never NULL. */
 const char* llama_engine_last_error(llama_engine_t engine);
 
 /* Device-resident greedy loop, equal to n_steps x { forward_token(tok, pos, 1); tok =
@@ -273,6 +273,92 @@ int llama_engine_debug_waits(llama_engine_t engine, unsigned long long wait_ns, 
  * without ordering) race; calls on one stream are safe.  n <= 16,777,216.  Returns 0, -1 on bad
  * arguments or a launch error, -2 when n exceeds the maximum. */
 int llama_b128_argmax_noalloc(const float* logits, int n, int32_t* out_index, void* stream);
+
+/* ---- paged KV cache and sampling on device memory (no counterpart in the reference) ---- */
+
+/* Element types of the operators below. */
+#define LLAMA_F32 0
+#define LLAMA_F16 1
+#define LLAMA_BF16 2
+
+/* A paged KV cache of one layer.  k and v are pools of num_pages pages of page_size rows; row r of
+ * page p holds head g at p * page_stride + r * row_stride + g * head_stride (elements; pages may
+ * lay their heads before or after their rows, and one pool may hold several layers).  Sequence s
+ * keeps key j in row j % page_size of page table[s * table_stride + j / page_size], for
+ * j < table_width * page_size.  Sequences may share pages that only attention reads.  A page id
+ * outside [0, num_pages) holds no rows: append writes nothing there, attention leaves its keys out.
+ * k, v and table are device memory; the calls read table on the device, so it may change between
+ * replays of a captured call. */
+typedef struct llama_paged_kv {
+  void* k;
+  void* v;
+  int32_t type;       /* LLAMA_F16 or LLAMA_BF16 */
+  int32_t num_pages;
+  int32_t page_size;  /* 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;
+  int32_t head_dim;   /* 64 or 128 */
+  int64_t page_stride, row_stride, head_stride; /* multiples of 8, at least head_dim */
+  const int32_t* table;
+  int32_t table_stride, table_width;
+  int32_t seqs;       /* rows of table */
+} llama_paged_kv_t;
+
+/* RoPE and cache append of `rows` tokens.  Row t of qkv (ld elements apart) is the token's q heads,
+ * k heads and v heads of head_dim elements each (the layout of the engine's q | k | v product);
+ * pos[t] is its position and seq[t] its sequence.  Writes the rotated q heads to row t of q_out
+ * (q_ld elements apart) and the rotated k and the v to the cache row of pos[t].  The rotation turns
+ * elements i and i + head_dim / 2 by row pos[t] of rope_cos / rope_sin ([n_pos][head_dim / 2], as
+ * llama_engine_rope_table makes them for head_dim 64), in fp32, rounded once.  type is LLAMA_F32 or
+ * the cache's type; q_type is type or the cache's type.  A row with seq[t] outside [0, seqs) or
+ * pos[t] outside [0, n_pos) is padding and writes nothing.  Of two rows with the same sequence and
+ * position, either may be the one kept.  qkv, q_out and the tables are 16-byte aligned, ld and q_ld
+ * multiples of 16 bytes.  Every pointer is memory of one device, which need not be the current one;
+ * the call is queued on `stream` (a cudaStream_t of that device) and may be captured.  Returns 0, or
+ * -1 on bad arguments or a launch error (llama_engine_last_error(NULL) says which). */
+int llama_paged_append(const llama_paged_kv_t* kv, const void* qkv, int type, int64_t ld, int rows, int heads,
+                       const int32_t* pos, const int32_t* seq, const float* rope_cos, const float* rope_sin,
+                       int n_pos, void* q_out, int q_type, int64_t q_ld, void* stream);
+
+/* Attention of new tokens over the cache.  Sequence s owns rows cu_q[s] .. cu_q[s + 1] - 1 of q and
+ * out (cu_q: seqs + 1 ascending values from 0, cu_q[seqs] <= rows) and kv_len[s] keys, its new tokens'
+ * included: row i of its n rows has position kv_len[s] - n + i and attends to keys 0 .. position.
+ * out = softmax(scale q . k) v per head, query head h reading kv head h / (heads / kv_heads); a row
+ * without a key (a position below 0, no valid page) is zeros; rows behind cu_q[seqs] are left as they
+ * were.  Keys past table_width * page_size do not exist: longer lengths count as that.  q has the
+ * cache's type, out_type is that or LLAMA_F32; scores, sums and the output accumulate in fp32, the
+ * softmax's weights enter the product with v in the cache's type.  max_q is at least every
+ * sequence's new tokens (a sequence of more may be left unwritten) and max_kv a bound of kv_len that
+ * only chooses how the work is split (any value is safe).  cu_q and kv_len are device memory, read
+ * on the device: a captured call may be replayed over other lengths.  q and out are 16-byte
+ * aligned and do not overlap, q_ld and out_ld multiples of 8.  workspace: 16-byte aligned device
+ * memory of at least llama_paged_attention_workspace(...) bytes for the same arguments (NULL where that
+ * is 0), whose contents need not be kept or cleared; calls that may overlap need one each.  Every
+ * pointer is memory of one device; queued on `stream`.  Returns 0, -1 on bad arguments or a
+ * launch error, -2 when the workspace is too small. */
+int llama_paged_attention(const llama_paged_kv_t* kv, const void* q, int64_t q_ld, int heads, const int32_t* cu_q,
+                          const int32_t* kv_len, int rows, int max_q, int max_kv, float scale, void* out,
+                          int out_type, int64_t out_ld, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that llama_paged_attention needs for these arguments (host only; 0 also for a
+ * descriptor that it would refuse). */
+size_t llama_paged_attention_workspace(const llama_paged_kv_t* kv, int heads, int rows, int max_q, int max_kv);
+
+/* One id for each of `rows` rows of logits (vocab values, ld apart, of `type`), written to out_ids.
+ * Per row: temperature (<= 0.01: the greedy id; NULL: 1), top_k (<= 0 or NULL: off), top_p (>= 1 or
+ * NULL: off), min_p (<= 0 or NULL: off) and uniform, a random number in [0, 1) (less or NaN counts
+ * as 0, more as the largest).  NaN in the other parameters turns a rule off (a temperature of NaN:
+ * greedy).  Logits <= -1e30 and NaN never win, as in llama_b128_argmax_noalloc; a row without any other gives 0.  With the ids
+ * ordered by logit, highest first, equal ones by index, and w = exp((logit - max) / temperature),
+ * each rule keeps a prefix: the first top_k; the fewest whose mass reaches top_p times the mass of
+ * the first top_k (at least one); those with w >= min_p.  The kept set is the shortest of them, and
+ * the id the first kept one, in index order, whose running mass exceeds uniform times the kept
+ * mass.  Masses are exact sums of weights rounded to 2^-44, so a row's id does not depend on the
+ * other rows, the grid or the order of sums.  All pointers are memory of one device; queued on
+ * `stream`, nothing is allocated.  Returns 0, -1 on bad arguments or a launch error, -2 for
+ * vocab > 262,144. */
+int llama_sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
+                      const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
+                      int32_t* out_ids, void* stream);
 
 #ifdef __cplusplus
 }

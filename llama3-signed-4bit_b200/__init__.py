@@ -10,8 +10,12 @@ The directory name is not a Python identifier; import it as ``llama3_signed_4bit
 """
 from . import build, convert, model_file, scoring, trace  # noqa: F401
 from .engine import (  # noqa: F401
+    BF16,
+    F16,
+    F32,
     LlamaEngine,
     LlamaEngineBindings,
+    PagedKV,
     TokenizerWrapper,
     ensure_library_built,
     tp_unique_id,

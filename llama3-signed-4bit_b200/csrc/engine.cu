@@ -32,6 +32,7 @@
 #include "tc_gemm.cuh"
 #include "attn_tc.cuh"
 #include "llama_engine.h"
+#include "ops.h"
 #include <nccl.h>
 
 #define LE_API extern "C" __attribute__((visibility("default")))
@@ -45,19 +46,7 @@ static void set_create_error(const std::string& s) {
   std::lock_guard<std::mutex> lk(g_err_mu);
   g_create_error = s;
 }
-
-// Restores the caller's current CUDA device on scope exit.
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-  }
-};
+void set_global_error(const std::string& s) { set_create_error(s); }
 
 struct FileMatrix {
   uint32_t N = 0, K = 0, nb = 0;

@@ -21,6 +21,18 @@ _P = ctypes.c_void_p
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _FP = ctypes.POINTER(ctypes.c_float)
 
+# element types of the paged-cache and sampling operators (include/llama_engine.h)
+F32, F16, BF16 = 0, 1, 2
+
+
+class PagedKV(ctypes.Structure):
+    """``llama_paged_kv_t``: a paged KV cache of one layer, on device memory."""
+    _fields_ = [("k", _P), ("v", _P), ("type", ctypes.c_int32), ("num_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("table", _P), ("table_stride", ctypes.c_int32), ("table_width", ctypes.c_int32),
+                ("seqs", ctypes.c_int32)]
+
 
 def ensure_library_built() -> Path:
     """Counterpart of ensure_dylib_built (src/main.py:27-46): builds the sm_100a library in-tree
@@ -113,6 +125,16 @@ class LlamaEngineBindings:
         lib.llama_engine_check_schedule.restype = ctypes.c_int
         lib.llama_engine_debug_waits.argtypes = [_P, ctypes.c_ulonglong, ctypes.c_int]
         lib.llama_engine_debug_waits.restype = ctypes.c_int
+        i32, i64, kvp = ctypes.c_int, ctypes.c_int64, ctypes.POINTER(PagedKV)
+        lib.llama_paged_append.argtypes = [kvp, _P, i32, i64, i32, i32, _P, _P, _P, _P, i32, _P, i32, i64, _P]
+        lib.llama_paged_append.restype = ctypes.c_int
+        lib.llama_paged_attention.argtypes = [kvp, _P, i64, i32, _P, _P, i32, i32, i32, ctypes.c_float, _P, i32, i64, _P,
+                                              ctypes.c_size_t, _P]
+        lib.llama_paged_attention.restype = ctypes.c_int
+        lib.llama_paged_attention_workspace.argtypes = [kvp, i32, i32, i32, i32]
+        lib.llama_paged_attention_workspace.restype = ctypes.c_size_t
+        lib.llama_sample_rows.argtypes = [_P, i32, i64, i32, i32, _P, _P, _P, _P, _P, _P, _P]
+        lib.llama_sample_rows.restype = ctypes.c_int
 
     def last_error(self, handle=None) -> str:
         return self.lib.llama_engine_last_error(handle).decode(errors="replace")
