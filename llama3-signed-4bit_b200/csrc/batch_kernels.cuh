@@ -52,13 +52,6 @@ __global__ void k_embed_batch(QMat E, const int32_t* __restrict__ tok, float* __
 constexpr int kAttnPart = 4 * 66;
 constexpr int kAttnRow = 68;
 constexpr int kAttnSmem = 2 * 3 * 32 * kAttnRow * 4;  // dynamic shared memory of k_attn_batch
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ float attn_sum_planes(const float* p, int nsplit, size_t stride) {
   return tc::sum_planes(p, nsplit, stride);
 }

@@ -1,0 +1,176 @@
+// Shared parts of the paged-cache kernels: the cache as they see it, element access, a sequence's
+// rows and keys, and the joining of key splits.
+//
+// The cache is a pool of pages of page_size rows; sequence s keeps key j in row j % page_size of
+// page table[s][j / page_size].  A page id outside [0, num_pages) holds no rows: nothing is
+// written there and its keys are left out of the softmax, so that a bad table cannot send an
+// access out of the pool.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace le {
+namespace paged {
+
+
+// What the kernels need of llama_paged_kv_t.
+struct Cache {
+  void* k;
+  void* v;
+  const int32_t* table;
+  int64_t page_stride, row_stride, head_stride;  // elements
+  int table_stride, table_width, seqs, num_pages, page_log2, kv_heads;
+};
+
+template <typename T> __device__ __forceinline__ float to_f32(T x);
+template <> __device__ __forceinline__ float to_f32(float x) { return x; }
+template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
+
+// 8 consecutive elements, 16-byte accesses (two for fp32).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint4 u;
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+    *reinterpret_cast<uint4*>(p) = u;
+  }
+}
+
+// Row of key j of sequence s in the pools (element offset of kv head g), or -1 when the table
+// holds no valid page for it.
+__device__ __forceinline__ int64_t key_offset(const Cache& C, int s, int j, int g) {
+  const int i = j >> C.page_log2;
+  if (i >= C.table_width) return -1;
+  const int page = C.table[(int64_t)s * C.table_stride + i];
+  if (page < 0 || page >= C.num_pages) return -1;
+  return (int64_t)page * C.page_stride + (int64_t)(j & ((1 << C.page_log2) - 1)) * C.row_stride +
+         (int64_t)g * C.head_stride;
+}
+
+// Two fp32 values rounded to T, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// 2^x (ex2.approx: 2^-22 relative; 2^-inf = 0).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Rows and keys of sequence s.  Rows outside [0, rows) and keys past the table do not exist.
+struct Span {
+  int first, n, len;  // first row, rows, keys
+};
+__device__ __forceinline__ Span span_of(const Cache& C, const int32_t* cu_q, const int32_t* kv_len, int s, int rows) {
+  Span x;
+  const int a = cu_q[s], b = cu_q[s + 1];
+  x.first = max(a, 0);
+  x.n = min(b, rows) - x.first;
+  // a clipped sequence keeps its rows' positions: rows cut off at the end take keys with them
+  x.len = max(0, min(kv_len[s], C.table_width << C.page_log2));
+  return x;
+}
+
+// Key splits that a sequence of len keys is cut into (at least one, which writes the zeros of a
+// sequence without keys).
+__host__ __device__ __forceinline__ int splits_of(int len, int per, int splits) {
+  const int u = (len + per - 1) / per;
+  return u < 1 ? 1 : u > splits ? splits : u;
+}
+
+// A split's part of a (row, head): D unnormalised outputs, then the maximum (log2 units) and sum.
+template <int D>
+__device__ __forceinline__ void write_part(float* part, int64_t index, int d, float m, float l, const float (&a)[8]) {
+  float* p = part + index * (D + 8);
+  store8(p + d, a);
+  if (d == 0) *reinterpret_cast<float2*>(p + D) = make_float2(m, l);
+}
+
+// out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the splits of a (row, head), M = max m_z.
+// D / 8 threads per (row, head); rows whose sequence has one split were written already.
+// splits / per: [0] sequences of at most small_rows query rows per kv head, [1] the others.
+struct SplitPlan {
+  int per[2], splits[2], small_rows;
+  int64_t part1;  // first part (index) of the second kind
+};
+template <typename O, int D>
+__global__ void __launch_bounds__(128)
+    k_paged_combine(Cache C, int heads, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ kv_len, int rows,
+                    SplitPlan P, const float* __restrict__ part, O* __restrict__ out, int64_t out_ld) {
+  grid_dep_wait();  // the parts come from the kernel before
+  constexpr int kRuns = D / 8;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t rh = i / kRuns;
+  if (rh >= (int64_t)rows * heads) return;
+  const int d = (int)(i % kRuns) * 8, t = (int)(rh / heads), h = (int)(rh % heads);
+  int lo = 0, hi = C.seqs;  // sequence of row t: the first whose end lies behind it
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu_q[mid + 1] <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  if (lo >= C.seqs) return;
+  const Span sp = span_of(C, cu_q, kv_len, lo, rows);
+  if (t < sp.first) return;
+  const int kind = sp.n * (heads / C.kv_heads) <= P.small_rows ? 0 : 1;
+  const int S = P.splits[kind], used = splits_of(sp.len, P.per[kind], S);
+  if (used <= 1) return;
+  const float* p = part + (rh * S + (kind ? P.part1 : 0)) * (D + 8);
+  float M = -INFINITY;
+  for (int z = 0; z < used; ++z) M = fmaxf(M, p[(int64_t)z * (D + 8) + D]);
+  float L = 0.0f, a[8] = {};
+  for (int z = 0; z < used; ++z) {
+    const float* pz = p + (int64_t)z * (D + 8);
+    const float2 ml = *reinterpret_cast<const float2*>(pz + D);
+    const float f = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - M);
+    float x[8];
+    load8(pz + d, x);
+    L = fmaf(ml.y, f, L);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = fmaf(x[e], f, a[e]);
+  }
+  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) a[e] *= inv;
+  store8(out + (int64_t)t * out_ld + (int64_t)h * D + d, a);
+}
+
+}  // namespace paged
+}  // namespace le

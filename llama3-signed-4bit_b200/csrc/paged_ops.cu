@@ -1,80 +1,22 @@
 // Paged KV cache operators behind the C ABI: llama_paged_append (RoPE and append) and
 // llama_paged_attention (attention of new tokens over the cache).
-//
-// The cache is a pool of pages of page_size rows; sequence s keeps key j in row j % page_size of
-// page table[s][j / page_size].  A page id outside [0, num_pages) holds no rows: nothing is
-// written there and its keys are left out of the softmax, so that a bad table cannot send an
-// access out of the pool.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cmath>
+#include <map>
+#include <mutex>
 
 #include "common.cuh"
 #include "ops.h"
+#include "paged.cuh"
+#include "paged_decode.cuh"
 
 #define LE_API extern "C" __attribute__((visibility("default")))
 
 namespace le {
 namespace paged {
-
-// What the kernels need of llama_paged_kv_t.
-struct Cache {
-  void* k;
-  void* v;
-  const int32_t* table;
-  int64_t page_stride, row_stride, head_stride;  // elements
-  int table_stride, table_width, seqs, num_pages, page_log2, kv_heads;
-};
-
-template <typename T> __device__ __forceinline__ float to_f32(T x);
-template <> __device__ __forceinline__ float to_f32(float x) { return x; }
-template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f32(float x);
-template <> __device__ __forceinline__ float from_f32(float x) { return x; }
-template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
-
-// 8 consecutive elements, 16-byte accesses (two for fp32).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
-    *reinterpret_cast<uint4*>(p) = u;
-  }
-}
-
-// Row of key j of sequence s in the pools (element offset of kv head g), or -1 when the table
-// holds no valid page for it.
-__device__ __forceinline__ int64_t key_offset(const Cache& C, int s, int j, int g) {
-  const int i = j >> C.page_log2;
-  if (i >= C.table_width) return -1;
-  const int page = C.table[(int64_t)s * C.table_stride + i];
-  if (page < 0 || page >= C.num_pages) return -1;
-  return (int64_t)page * C.page_stride + (int64_t)(j & ((1 << C.page_log2) - 1)) * C.row_stride +
-         (int64_t)g * C.head_stride;
-}
 
 // ---------------------------------------------------------------------------------------------
 // Append.  Row t of qkv is q heads | k heads | v heads; with (c, s) the table row of its position,
@@ -133,7 +75,8 @@ __global__ void __launch_bounds__(256)
 template <typename T, typename O, int D>
 __global__ void __launch_bounds__(128)
     k_paged_attention(Cache C, const T* __restrict__ q, int64_t q_ld, int heads, const int32_t* __restrict__ cu_q,
-                      const int32_t* __restrict__ kv_len, int rows, float scale, O* __restrict__ out, int64_t out_ld) {
+                      const int32_t* __restrict__ kv_len, int rows, float scale, int small_rows,
+                      O* __restrict__ out, int64_t out_ld) {
   constexpr int kE = D / 32;
   const int lane = threadIdx.x & 31;
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
@@ -147,6 +90,7 @@ __global__ void __launch_bounds__(128)
   }
   if (lo >= C.seqs || t < cu_q[lo]) return;  // a row behind the last sequence
   const int s = lo, g = h / (heads / C.kv_heads);
+  if ((cu_q[s + 1] - cu_q[s]) * (heads / C.kv_heads) <= small_rows) return;
   const int last = min(kv_len[s], C.table_width << C.page_log2) - (cu_q[s + 1] - t);
   float qv[kE], o[kE], m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -272,9 +216,103 @@ LE_API int llama_paged_append(const llama_paged_kv_t* kv, const void* qkv, int t
   return e == cudaSuccess ? 0 : refuse(who, cudaGetErrorString(e));
 }
 
+namespace le {
+namespace paged {
+
+constexpr int kSms = 148;  // the workspace's size must not need a device
+
+// How a call is cut: which kernels run, and their key splits.
+struct Plan {
+  SplitPlan sp{};
+  bool decode = false, chunk = false;
+  size_t bytes = 0;
+};
+static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, int max_kv) {
+  Plan P;
+  const int G = heads / kv->kv_heads;
+  const int64_t keys = std::max<int64_t>(1, std::min<int64_t>(max_kv, (int64_t)kv->table_width * kv->page_size));
+  P.chunk = (int64_t)max_q * G > kDecodeRows;
+  // beside chunks there are sequences of few tokens unless all have max_q of them
+  P.decode = !P.chunk || (kv->seqs > 1 && rows < (int64_t)kv->seqs * max_q && G <= kDecodeRows);
+  P.sp.small_rows = P.decode ? kDecodeRows : 0;
+  const int64_t units = (int64_t)std::min(kv->seqs, std::max(rows, 1)) * kv->kv_heads;
+  // decode: about eight CTAs for every SM where the keys allow, of 64 keys (one slice for each warp) at least
+  int64_t per = (units * keys + kSms * 8 - 1) / (kSms * 8);
+  per = std::max<int64_t>(64, (per + 63) / 64 * 64);
+  P.sp.per[0] = (int)per;
+  P.sp.splits[0] = P.decode ? (int)((keys + per - 1) / per) : 1;
+  P.sp.per[1] = 1 << 30;
+  P.sp.splits[1] = 1;
+  const int64_t pairs = (int64_t)rows * heads;
+  const int64_t n0 = P.sp.splits[0] > 1 ? pairs * P.sp.splits[0] : 0, n1 = P.sp.splits[1] > 1 ? pairs * P.sp.splits[1] : 0;
+  P.sp.part1 = n0;
+  P.bytes = (size_t)(n0 + n1) * (kv->head_dim + 8) * sizeof(float);
+  return P;
+}
+
+// Dynamic shared memory above 48 KB, allowed once per kernel and device.
+template <typename F>
+static bool allow_smem(F* fn, int bytes, int dev) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, bool> done;
+  std::lock_guard<std::mutex> lk(mu);
+  bool& d = done[{reinterpret_cast<const void*>(fn), dev}];
+  if (!d) d = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  return d;
+}
+
+// A launch that may start while the kernel before it runs out; that kernel's results are there
+// after its griddepcontrol.wait.
+template <typename... KArgs, typename... Args>
+static void launch(bool early, void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
+                   Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+template <typename T, typename O, int D>
+static const char* attention(const Plan& P, const Cache& C, int dev, const void* q, int64_t q_ld, int heads,
+                             const int32_t* cu_q, const int32_t* kv_len, int rows, float scale, void* out,
+                             int64_t out_ld, float* part, cudaStream_t st) {
+  const T* qt = static_cast<const T*>(q);
+  O* ot = static_cast<O*>(out);
+  if (P.chunk) {
+    const int64_t grid = ((int64_t)rows * heads + 3) / 4;
+    k_paged_attention<T, O, D><<<(unsigned)grid, 128, 0, st>>>(C, qt, q_ld, heads, cu_q, kv_len, rows, scale,
+                                                               P.sp.small_rows, ot, out_ld);
+  }
+  if (P.decode) {
+    const int64_t grid = (int64_t)C.seqs * C.kv_heads * P.sp.splits[0];
+    if (grid > 0x7fffffff) return "too many sequences";
+    if (!allow_smem(k_paged_decode<T, O, D>, DecodeGeo<D>::kSmem, dev)) return "shared memory could not be set";
+    launch(P.chunk, k_paged_decode<T, O, D>, (unsigned)grid, 32 * kDecodeWarps, DecodeGeo<D>::kSmem, st, C, qt, q_ld,
+           heads, cu_q, kv_len, rows, scale * 1.44269504f, P.sp.per[0], P.sp.splits[0], ot, out_ld, part);
+  }
+  if (P.sp.splits[0] > 1 || P.sp.splits[1] > 1) {
+    const int64_t grid = ((int64_t)rows * heads * (D / 8) + 127) / 128;
+    if (grid > 0x7fffffff) return "too many rows";
+    launch(true, k_paged_combine<O, D>, (unsigned)grid, 128, 0, st, C, heads, cu_q, kv_len, rows, P.sp, part, ot, out_ld);
+  }
+  return nullptr;
+}
+
+}  // namespace paged
+}  // namespace le
+
 LE_API size_t llama_paged_attention_workspace(const llama_paged_kv_t* kv, int heads, int rows, int max_q, int max_kv) {
-  (void)heads; (void)rows; (void)max_q; (void)max_kv;
-  return paged::check_cache(kv) ? 0 : 16;
+  using namespace paged;
+  if (check_cache(kv) || heads < 1 || heads > 4096 || heads % kv->kv_heads != 0 || rows < 1 || max_q < 0 || max_kv < 0)
+    return 0;
+  return plan_of(kv, heads, rows, max_q, max_kv).bytes;
 }
 
 LE_API int llama_paged_attention(const llama_paged_kv_t* kv, const void* q, int64_t q_ld, int heads,
@@ -293,31 +331,25 @@ LE_API int llama_paged_attention(const llama_paged_kv_t* kv, const void* q, int6
   if (q_ld < (int64_t)heads * D || q_ld % 8 != 0) return refuse(who, "q_ld is shorter than a row or not a multiple of 8");
   if (out_ld < (int64_t)heads * D || out_ld % 8 != 0) return refuse(who, "out_ld is shorter than a row or not a multiple of 8");
   if (!aligned16(q) || !aligned16(out)) return refuse(who, "q and out must be 16-byte aligned");
-  const size_t need = llama_paged_attention_workspace(kv, heads, rows, max_q, max_kv);
-  if (need > 16 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
-    return refuse(who, "workspace is too small", -2);
   if (rows == 0) return 0;
+  const Plan P = plan_of(kv, heads, rows, max_q, max_kv);
+  if (P.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < P.bytes))
+    return refuse(who, "workspace is too small", -2);
   const int dev = device_of(kv->k);
-  const void* ptrs[] = {kv->v, kv->table, q, cu_q, kv_len, out};
+  const void* ptrs[] = {kv->v, kv->table, q, cu_q, kv_len, out, workspace};
   for (const void* p : ptrs)
-    if (dev < 0 || device_of(p) != dev) return refuse(who, "every pointer must be memory of one CUDA device");
+    if (dev < 0 || (p && device_of(p) != dev)) return refuse(who, "every pointer must be memory of one CUDA device");
   DeviceGuard dg(dev);
   const Cache C = cache_of(kv);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)(((int64_t)rows * heads + 3) / 4);
-  auto launch = [&](auto c, auto o) {
+  auto run = [&](auto c, auto o) {
     using T = decltype(c);
     using O = decltype(o);
-    auto* fn = D == 64 ? k_paged_attention<T, O, 64> : k_paged_attention<T, O, 128>;
-    fn<<<grid, 128, 0, st>>>(C, static_cast<const T*>(q), q_ld, heads, cu_q, kv_len, rows, scale, static_cast<O*>(out),
-                             out_ld);
+    auto* fn = D == 64 ? attention<T, O, 64> : attention<T, O, 128>;
+    return fn(P, C, dev, q, q_ld, heads, cu_q, kv_len, rows, scale, out, out_ld, static_cast<float*>(workspace),
+              static_cast<cudaStream_t>(stream));
   };
-  auto by_type = [&](auto c) {
-    if (out_type == LLAMA_F32) launch(c, 0.0f);
-    else launch(c, c);
-  };
-  if (kv->type == LLAMA_F16) by_type(__half{});
-  else by_type(__nv_bfloat16{});
+  auto by_type = [&](auto c) { return out_type == LLAMA_F32 ? run(c, 0.0f) : run(c, c); };
+  if (const char* why = kv->type == LLAMA_F16 ? by_type(__half{}) : by_type(__nv_bfloat16{})) return refuse(who, why);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : refuse(who, cudaGetErrorString(e));
 }
