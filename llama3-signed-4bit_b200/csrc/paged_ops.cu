@@ -11,6 +11,7 @@
 #include "common.cuh"
 #include "ops.h"
 #include "paged.cuh"
+#include "paged_chunk.cuh"
 #include "paged_decode.cuh"
 
 #define LE_API extern "C" __attribute__((visibility("default")))
@@ -66,58 +67,6 @@ __global__ void __launch_bounds__(256)
   Kv* dst = static_cast<Kv*>(is_k ? C.k : C.v) + off + i0;
   store8(dst, a);
   store8(dst + D / 2, b);
-}
-
-// ---------------------------------------------------------------------------------------------
-// Attention: o = sum_j p_j v_j with p = softmax(scale q . k_j) over the keys 0 .. position of the
-// token, one pass with a running maximum and sum (fp32).  One warp per (token, head).
-// ---------------------------------------------------------------------------------------------
-template <typename T, typename O, int D>
-__global__ void __launch_bounds__(128)
-    k_paged_attention(Cache C, const T* __restrict__ q, int64_t q_ld, int heads, const int32_t* __restrict__ cu_q,
-                      const int32_t* __restrict__ kv_len, int rows, float scale, int small_rows,
-                      O* __restrict__ out, int64_t out_ld) {
-  constexpr int kE = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  if (w >= (int64_t)rows * heads) return;
-  const int t = (int)(w / heads), h = (int)(w % heads);
-  int lo = 0, hi = C.seqs;  // sequence of row t: cu_q[lo] <= t < cu_q[lo + 1]
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cu_q[mid + 1] <= t) lo = mid + 1;
-    else hi = mid;
-  }
-  if (lo >= C.seqs || t < cu_q[lo]) return;  // a row behind the last sequence
-  const int s = lo, g = h / (heads / C.kv_heads);
-  if ((cu_q[s + 1] - cu_q[s]) * (heads / C.kv_heads) <= small_rows) return;
-  const int last = min(kv_len[s], C.table_width << C.page_log2) - (cu_q[s + 1] - t);
-  float qv[kE], o[kE], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int e = 0; e < kE; ++e) {
-    qv[e] = to_f32(q[(int64_t)t * q_ld + (int64_t)h * D + lane * kE + e]) * scale;
-    o[e] = 0.0f;
-  }
-  for (int j = 0; j <= last; ++j) {
-    const int64_t off = key_offset(C, s, j, g);
-    if (off < 0) continue;
-    const T* kr = static_cast<const T*>(C.k) + off + lane * kE;
-    const T* vr = static_cast<const T*>(C.v) + off + lane * kE;
-    float d = 0.0f;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) d = fmaf(qv[e], to_f32(kr[e]), d);
-    d = warp_sum(d);
-    if (d == -INFINITY) continue;
-    const float mn = fmaxf(m, d);
-    const float alpha = expf(m - mn), p = expf(d - mn);
-    l = l * alpha + p;
-    m = mn;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = fmaf(o[e], alpha, p * to_f32(vr[e]));
-  }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // no key: zeros
-#pragma unroll
-  for (int e = 0; e < kE; ++e) out[(int64_t)t * out_ld + (int64_t)h * D + lane * kE + e] = from_f32<O>(o[e] * inv);
 }
 
 static int refuse(const char* what, const char* why, int rc = -1) {
@@ -241,8 +190,23 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   per = std::max<int64_t>(64, (per + 63) / 64 * 64);
   P.sp.per[0] = (int)per;
   P.sp.splits[0] = P.decode ? (int)((keys + per - 1) / per) : 1;
+  // chunk: one CTA per SM; as many splits as make the estimated waves x (a split's keys + the fixed
+  // cost of an item, about that of 256 keys) smallest, at least 512 keys each
   P.sp.per[1] = 1 << 30;
   P.sp.splits[1] = 1;
+  if (P.chunk) {
+    const int64_t items = std::max<int64_t>(1, ((int64_t)rows * G + kItemRows - 1) / kItemRows) * kv->kv_heads;
+    int64_t best = -1;
+    for (int64_t n = 1; n <= 32 && (n == 1 || keys >= 512 * n); ++n) {
+      const int64_t p1 = (keys + n * kTileKeys - 1) / (n * kTileKeys) * kTileKeys;
+      const int64_t cost = (items * n + kSms - 1) / kSms * (p1 + 256);
+      if (best < 0 || cost < best) {
+        best = cost;
+        P.sp.per[1] = n == 1 ? 1 << 30 : (int)p1;
+        P.sp.splits[1] = (int)((keys + p1 - 1) / p1);
+      }
+    }
+  }
   const int64_t pairs = (int64_t)rows * heads;
   const int64_t n0 = P.sp.splits[0] > 1 ? pairs * P.sp.splits[0] : 0, n1 = P.sp.splits[1] > 1 ? pairs * P.sp.splits[1] : 0;
   P.sp.part1 = n0;
@@ -279,16 +243,59 @@ static void launch(bool early, void (*kernel)(KArgs...), unsigned grid, unsigned
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// TMA map of a pool: (element, head, row, page), boxes of 64 elements x one head x up to 128 rows of a
+// page, 128-byte swizzle.
+static bool pool_map(CUtensorMap* m, const llama_paged_kv_t* kv, void* pool) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult st;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &st) != cudaSuccess) fn = nullptr;
+    return reinterpret_cast<Encode>(fn);
+  }();
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)kv->head_dim, (cuuint64_t)kv->kv_heads, (cuuint64_t)kv->page_size,
+                              (cuuint64_t)kv->num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)kv->head_stride * 2, (cuuint64_t)kv->row_stride * 2,
+                                 (cuuint64_t)kv->page_stride * 2};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)std::min(kv->page_size, kTileKeys), 1};
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return encode(m, kv->type == LLAMA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool, dims,
+                strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Device word that a wait which ran out in the chunk form sets (its rows become NaN as well).
+__device__ uint32_t g_paged_error;
+static uint32_t* error_word(int dev) {
+  static std::mutex mu;
+  static std::map<int, uint32_t*> at;
+  std::lock_guard<std::mutex> lk(mu);
+  uint32_t*& p = at[dev];
+  if (!p && cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_paged_error) != cudaSuccess) p = nullptr;
+  return p;
+}
+
 template <typename T, typename O, int D>
-static const char* attention(const Plan& P, const Cache& C, int dev, const void* q, int64_t q_ld, int heads,
+static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Cache& C, int dev, const void* q, int64_t q_ld, int heads,
                              const int32_t* cu_q, const int32_t* kv_len, int rows, float scale, void* out,
                              int64_t out_ld, float* part, cudaStream_t st) {
   const T* qt = static_cast<const T*>(q);
   O* ot = static_cast<O*>(out);
   if (P.chunk) {
-    const int64_t grid = ((int64_t)rows * heads + 3) / 4;
-    k_paged_attention<T, O, D><<<(unsigned)grid, 128, 0, st>>>(C, qt, q_ld, heads, cu_q, kv_len, rows, scale,
-                                                               P.sp.small_rows, ot, out_ld);
+    const int G = heads / C.kv_heads;
+    const int64_t items = ((int64_t)rows * G + kItemRows - 1) / kItemRows + std::min(C.seqs, rows);
+    const int64_t grid = items * C.kv_heads * P.sp.splits[1];
+    if (grid > 0x7fffffff) return "too many rows";
+    CUtensorMap mk, mv;
+    uint32_t* err = error_word(dev);
+    if (!err || !pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v)) return "tensor maps of the pools could not be made";
+    if (!allow_smem(k_paged_chunk<T, O, D>, ChunkGeo<D>::kSmem, dev)) return "shared memory could not be set";
+    launch(false, k_paged_chunk<T, O, D>, (unsigned)grid, kChunkThreads, ChunkGeo<D>::kSmem, st, mk, mv, C, qt, q_ld, heads,
+           cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], ot, out_ld,
+           part + P.sp.part1 * (D + 8), err);
   }
   if (P.decode) {
     const int64_t grid = (int64_t)C.seqs * C.kv_heads * P.sp.splits[0];
@@ -345,7 +352,7 @@ LE_API int llama_paged_attention(const llama_paged_kv_t* kv, const void* q, int6
     using T = decltype(c);
     using O = decltype(o);
     auto* fn = D == 64 ? attention<T, O, 64> : attention<T, O, 128>;
-    return fn(P, C, dev, q, q_ld, heads, cu_q, kv_len, rows, scale, out, out_ld, static_cast<float*>(workspace),
+    return fn(kv, P, C, dev, q, q_ld, heads, cu_q, kv_len, rows, scale, out, out_ld, static_cast<float*>(workspace),
               static_cast<cudaStream_t>(stream));
   };
   auto by_type = [&](auto c) { return out_type == LLAMA_F32 ? run(c, 0.0f) : run(c, c); };
