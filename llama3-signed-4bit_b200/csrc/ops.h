@@ -6,7 +6,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <map>
+#include <mutex>
 #include <string>
+#include <utility>
 
 #include "llama_engine.h"
 
@@ -36,6 +39,17 @@ inline int device_of(const void* p) {
     return -1;
   }
   return a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged ? a.device : -1;
+}
+
+// Dynamic shared memory above 48 KB, allowed once per kernel and device.
+template <typename F>
+inline bool allow_smem(F* fn, int bytes, int dev) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, bool> done;
+  std::lock_guard<std::mutex> lk(mu);
+  bool& d = done[{reinterpret_cast<const void*>(fn), dev}];
+  if (!d) d = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  return d;
 }
 
 }  // namespace le

@@ -214,17 +214,6 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   return P;
 }
 
-// Dynamic shared memory above 48 KB, allowed once per kernel and device.
-template <typename F>
-static bool allow_smem(F* fn, int bytes, int dev) {
-  static std::mutex mu;
-  static std::map<std::pair<const void*, int>, bool> done;
-  std::lock_guard<std::mutex> lk(mu);
-  bool& d = done[{reinterpret_cast<const void*>(fn), dev}];
-  if (!d) d = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
-  return d;
-}
-
 // A launch that may start while the kernel before it runs out; that kernel's results are there
 // after its griddepcontrol.wait.
 template <typename... KArgs, typename... Args>
