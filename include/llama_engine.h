@@ -105,6 +105,26 @@ const char* llama_tokenizer_decode(llama_tokenizer_t tokenizer, int32_t token_id
  * 8192).  Slot 0 is the sequence used by the Part-1 calls.  NULL on failure. */
 llama_engine_t llama_engine_create_ex(const char* model_path, int device, int max_batch, int max_seq_len);
 
+/* Like llama_engine_create_ex, with a paged KV cache: all slots share a pool of num_pages pages of
+ * page_size positions (16, 32, 64, 128 or 256) in cache_type (LLAMA_F16 or LLAMA_BF16), instead of fp32
+ * rows for max_seq_len positions of every slot (half the bytes per position, and only for
+ * positions in use).  A page is given out when one of its positions is first fed, and returned by
+ * llama_engine_release_slot; a call that needs more pages than are free fails (-1) before it queues
+ * anything.  Keys, values and rotated queries are rounded to cache_type, so logits differ from the
+ * fp32 cache's by that rounding.  Needs the tensor-core batched path; every step runs on it,
+ * forward_token and generate_greedy as steps of one row.  A position that was never fed holds no key
+ * (positions of a page that was given out for a neighbour hold stale ones: feed a sequence in order).
+ * profile_phase is not available.  NULL on failure. */
+llama_engine_t llama_engine_create_paged(const char* model_path, int device, int max_batch, int max_seq_len,
+                                         int num_pages, int page_size, int cache_type);
+
+/* Returns the pages of a slot of a paged engine to the pool, behind the work already queued; the slot
+ * starts anew.  Returns 0, or -1 on bad arguments. */
+int llama_engine_release_slot(llama_engine_t engine, int slot);
+
+/* Pages of a paged engine that no slot holds; -1 for a NULL handle or an engine without pages. */
+int llama_engine_free_pages(llama_engine_t engine);
+
 /* Message of the last failure on this handle (or, when engine is NULL, of the last failed create
  * or the last refused llama_paged_* / llama_sample_rows call).  Never NULL. */
 const char* llama_engine_last_error(llama_engine_t engine);
@@ -130,6 +150,16 @@ int llama_engine_forward_batch(llama_engine_t engine, const int32_t* tokens, con
 /* Greedy ids (first index among equal maxima) of the n rows of the last forward_batch.
  * Waits for the step; -1 on bad arguments or a device error. */
 int llama_engine_argmax_batch(llama_engine_t engine, int32_t* out_tokens, int n);
+
+/* One id for each of rows 0 .. n - 1 of the last forward_batch with logits, drawn on the device under the
+ * row's own rules from the given random numbers: host arrays of n values, read as in
+ * llama_sample_rows (any but uniform may be NULL: off; temperature <= 0.01 or a row of masked logits:
+ * greedy).  Row 0 is also what forward_token, prefill and score_tokens leave as the current logits.
+ * The logits are not changed (llama_engine_sample with a temperature replaces row 0's by
+ * probabilities).  Waits for the step.  n <= max_batch and the vocabulary at most 262,144 ids.
+ * Returns 0, or -1 on bad arguments or a device error. */
+int llama_engine_sample_batch(llama_engine_t engine, const float* temperature, const int32_t* top_k, const float* top_p,
+                              const float* min_p, const float* uniform, int n, int32_t* out_tokens);
 
 /* Host pointer to the logits of row `row` of the last forward_batch (vocab_size floats,
  * refreshed by this call).  NULL on error. */
@@ -287,8 +317,10 @@ int llama_b128_argmax_noalloc(const float* logits, int n, int32_t* out_index, vo
  * keeps key j in row j % page_size of page table[s * table_stride + j / page_size], for
  * j < table_width * page_size.  Sequences may share pages that only attention reads.  A page id
  * outside [0, num_pages) holds no rows: append writes nothing there, attention leaves its keys out.
- * k, v and table are device memory; the calls read table on the device, so it may change between
- * replays of a captured call. */
+ * With slots, "table[s]" is table[slots[s]] (a batch whose sequences lie anywhere in a larger table;
+ * two sequences of an attention call may name the same row); a value outside [0, table_rows) has no
+ * pages.  k, v, table and slots are device memory; the calls read table and slots on the device, so
+ * they may change between replays of a captured call. */
 typedef struct llama_paged_kv {
   void* k;
   void* v;
@@ -300,7 +332,9 @@ typedef struct llama_paged_kv {
   int64_t page_stride, row_stride, head_stride; /* multiples of 8, at least head_dim */
   const int32_t* table;
   int32_t table_stride, table_width;
-  int32_t seqs;       /* rows of table */
+  int32_t seqs;              /* sequences of the call */
+  const int32_t* slots;      /* NULL: sequence s has row s of table; else device memory: row slots[s] */
+  int32_t table_rows;        /* rows of table with slots, 0 without */
 } llama_paged_kv_t;
 
 /* RoPE and cache append of `rows` tokens.  Row t of qkv (ld elements apart) is the token's q heads,
@@ -329,7 +363,8 @@ int llama_paged_append(const llama_paged_kv_t* kv, const void* qkv, int type, in
  * softmax's weights enter the product with v in the cache's type.  max_q is at least every
  * sequence's new tokens (a sequence of more may be left unwritten) and max_kv a bound of kv_len that
  * only chooses how the work is split (any value is safe).  cu_q and kv_len are device memory, read
- * on the device: a captured call may be replayed over other lengths.  q and out are 16-byte
+ * on the device: a captured call may be replayed over other lengths.  Keys and values of a
+ * sequence's kv_len keys are finite; rows of its last page behind them may hold anything.  q and out are 16-byte
  * aligned and do not overlap, q_ld and out_ld multiples of 8.  workspace: 16-byte aligned device
  * memory of at least llama_paged_attention_workspace(...) bytes for the same arguments (NULL where that
  * is 0), whose contents need not be kept or cleared; calls that may overlap need one each.  Every

@@ -246,13 +246,27 @@ struct Engine {
   unsigned long long attn_wait_ns = kWaitNs;  // bound on the prefill attention's waits (test hook)
   // decode steps of the batched path replayed as CUDA graphs, one per (rows, logits rows,
   // attention splits); the rows' ids, positions and slots are read from t_idx
-  struct TcGraph { int n, nlog, splits; bool fold; cudaGraphExec_t exec; };
+  struct TcGraph { int n, nlog, splits; bool fold; int runs, run_q, run_kv; cudaGraphExec_t exec; };
   std::vector<TcGraph> tc_graphs;
   // token scoring (llama_engine_score_tokens): logits of a chunk's rows, targets, results
   float* sc_logits = nullptr;   // [kScoreRows][vocab], allocated on first use
   int32_t* sc_target = nullptr; // [kScoreRows]
   float* sc_lp = nullptr;       // [kScoreRows]
   int32_t* sc_greedy = nullptr; // [kScoreRows]
+
+  // paged KV cache (llama_engine_create_paged): one pool for all slots, pages given out as positions
+  // are first fed; a step's rows are cut into runs (consecutive positions of one slot)
+  bool paged = false;
+  int page_size = 0, num_pages = 0, page_type = 0, page_width = 0;  // page_width: table entries per slot
+  uint8_t* pool_k = nullptr;     // [layer][page][page_size][kv_dim], 16-bit
+  uint8_t* pool_v = nullptr;
+  int32_t* d_table = nullptr;    // [max_batch][page_width]
+  std::vector<int32_t> h_table, free_pages;
+  uint8_t* paged_ws = nullptr;   // attention workspace
+  int runs = 0, run_q = 0, run_kv = 0;  // of the uploaded step: runs, bounds of their rows and keys
+  // batched sampling (llama_engine_sample_batch): 5 parameters and the id of each row
+  int32_t* d_sample = nullptr;   // [6][max_batch]
+  int32_t* h_sample = nullptr;
 
   cudaGraphExec_t g_fwd[2] = {nullptr, nullptr};  // [compute_logits]
   cudaGraphExec_t g_gen = nullptr;                // forward + greedy + advance
@@ -773,6 +787,7 @@ static bool tc_supported(const Engine* E) {
   return E->dim % 2048 == 0 && E->ffn % 2048 == 0 && E->heads == 4 * E->kv_heads;
 }
 
+static size_t idx_words(const Engine* E);
 static bool init_tc(Engine* E) {
   if (!tc_supported(E)) return true;
   using namespace tc;
@@ -836,10 +851,12 @@ static bool init_tc(Engine* E) {
   LE_CK(cudaMalloc(&E->t_gu, (size_t)T * ffn * 4));
   LE_CK(cudaMalloc(&E->t_part, (size_t)kTcMaxSplits * T * dim * 4));
   LE_CK(cudaMalloc(&E->t_attn_part, (size_t)T * E->kv_heads * kAttnMaxSplits * kAttnPart * 4));
-  E->kv_img_tiles = (E->max_seq + attn::kKeys - 1) / attn::kKeys;
-  LE_CK(cudaMalloc(&E->kv_img, (size_t)E->kv_heads * E->kv_img_tiles * attn::kTileBytes));
-  LE_CK(cudaMalloc(&E->t_idx, (size_t)3 * T * 4));
-  LE_CK(cudaMallocHost(&E->h_idx, (size_t)3 * T * 4));
+  if (!E->paged) {
+    E->kv_img_tiles = (E->max_seq + attn::kKeys - 1) / attn::kKeys;
+    LE_CK(cudaMalloc(&E->kv_img, (size_t)E->kv_heads * E->kv_img_tiles * attn::kTileBytes));
+  }
+  LE_CK(cudaMalloc(&E->t_idx, idx_words(E) * 4));
+  LE_CK(cudaMallocHost(&E->h_idx, idx_words(E) * 4));
   LE_CK(cudaEventCreateWithFlags(&E->idx_ev, cudaEventDisableTiming));
   E->tc_am_parts = std::min<int>(64, ((int)E->vocab + 4 * 256 - 1) / (4 * 256));
   LE_CK(cudaMalloc(&E->t_am, (size_t)T * E->tc_am_parts * sizeof(ArgmaxPart)));
@@ -970,6 +987,116 @@ static bool tc_upload_rows(Engine* E, const int32_t* tok, const int32_t* pos, co
   return true;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Paged KV cache of an engine: pages for the rows' positions, and the rows as runs.
+// ---------------------------------------------------------------------------------------------
+__global__ void k_page_updates(int32_t* __restrict__ table, const int32_t* __restrict__ at,
+                               const int32_t* __restrict__ page, int n) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) table[at[i]] = page[i];
+}
+
+// Layout of t_idx for a paged step of n rows in r runs, behind token | position | slot: run of each
+// row [n], first row of each run [r + 1], keys of each run [r], slot of each run [r], then the table
+// updates.
+static size_t idx_words(const Engine* E) { return E->paged ? (size_t)9 * E->tc_T + 16 : (size_t)3 * E->tc_T; }
+
+static llama_paged_kv_t paged_desc(const Engine* E, int n, uint32_t layer) {
+  llama_paged_kv_t kv{};
+  const size_t layer_bytes = (size_t)E->num_pages * E->page_size * E->kv_dim * 2;
+  kv.k = E->pool_k + layer * layer_bytes;
+  kv.v = E->pool_v + layer * layer_bytes;
+  kv.type = E->page_type;
+  kv.num_pages = E->num_pages;
+  kv.page_size = E->page_size;
+  kv.kv_heads = (int32_t)E->kv_heads;
+  kv.head_dim = LE_HEAD_DIM;
+  kv.page_stride = (int64_t)E->page_size * E->kv_dim;
+  kv.row_stride = E->kv_dim;
+  kv.head_stride = LE_HEAD_DIM;
+  kv.table = E->d_table;
+  kv.table_stride = kv.table_width = E->page_width;
+  kv.seqs = E->runs;
+  kv.slots = E->t_idx + 4 * n + E->runs + 1 + E->runs;
+  kv.table_rows = E->max_batch;
+  return kv;
+}
+
+// Are there pages for `count` positions of slot 0 from `start` on?  Asked before the first chunk of a
+// call that runs several.
+static bool pages_fit(Engine* E, size_t start, size_t count) {
+  if (!E->paged || count == 0) return true;
+  size_t need = 0;
+  for (size_t i = start / E->page_size; i <= (start + count - 1) / E->page_size; ++i) need += E->h_table[i] < 0 ? 1 : 0;
+  if (need <= E->free_pages.size()) return true;
+  E->err = "out of KV cache pages (release slots, or create the engine with more pages)";
+  return false;
+}
+
+// Gives the rows' positions their pages (all of them or none) and uploads the step's rows.
+static bool paged_upload_rows(Engine* E, const int32_t* tok, const int32_t* pos, const int32_t* slot, int n) {
+  std::vector<int32_t> fresh;  // table entries that get a page
+  for (int i = 0; i < n; ++i) {
+    int32_t& e = E->h_table[(size_t)slot[i] * E->page_width + pos[i] / E->page_size];
+    if (e == -1) {
+      e = -2;
+      fresh.push_back((int32_t)(&e - E->h_table.data()));
+    }
+  }
+  if (fresh.size() > E->free_pages.size()) {
+    for (int32_t at : fresh) E->h_table[at] = -1;
+    E->err = "out of KV cache pages (release slots, or create the engine with more pages)";
+    return false;
+  }
+  for (int32_t at : fresh) {
+    E->h_table[at] = E->free_pages.back();
+    E->free_pages.pop_back();
+  }
+  if (E->idx_pending) LE_CK(cudaEventSynchronize(E->idx_ev));
+  std::vector<int32_t> first, keys, slots;
+  int longest = 0, most = 0;
+  int32_t* h = E->h_idx;
+  for (int i = 0; i < n; ++i) {
+    h[i] = tok[i] < 0 || tok[i] >= (int32_t)E->vocab ? 0 : tok[i];  // src/llama_engine.cpp:937
+    h[n + i] = pos[i];
+    h[2 * n + i] = slot[i];
+    if (i == 0 || slot[i] != slot[i - 1] || pos[i] != pos[i - 1] + 1) {
+      first.push_back(i);
+      keys.push_back(0);
+      slots.push_back(slot[i]);
+    }
+    keys.back() = pos[i] + 1;
+    h[3 * n + i] = (int32_t)first.size() - 1;
+    longest = std::max(longest, i - first.back() + 1);
+    most = std::max(most, pos[i] + 1);
+  }
+  E->runs = (int)first.size();
+  // bounds rounded up, so that few of them (and few captured steps) exist
+  for (E->run_q = 1; E->run_q < longest;) E->run_q *= 2;
+  for (E->run_kv = 256; E->run_kv < most;) E->run_kv *= 2;
+  first.push_back(n);
+  int32_t* at = h + 4 * n;
+  at = std::copy(first.begin(), first.end(), at);
+  at = std::copy(keys.begin(), keys.end(), at);
+  at = std::copy(slots.begin(), slots.end(), at);
+  const size_t upd = (size_t)(at - h);
+  at = std::copy(fresh.begin(), fresh.end(), at);
+  for (int32_t f : fresh) *at++ = E->h_table[f];
+  LE_CK(cudaMemcpyAsync(E->t_idx, h, (size_t)(at - h) * 4, cudaMemcpyHostToDevice, E->stream));
+  LE_CK(cudaEventRecord(E->idx_ev, E->stream));
+  E->idx_pending = true;
+  if (!fresh.empty()) {
+    const int f = (int)fresh.size();
+    k_page_updates<<<(f + 255) / 256, 256, 0, E->stream>>>(E->d_table, E->t_idx + upd, E->t_idx + upd + f, f);
+    LE_CK(cudaGetLastError());
+  }
+  return true;
+}
+
+static bool upload_rows(Engine* E, const int32_t* tok, const int32_t* pos, const int32_t* slot, int n) {
+  return E->paged ? paged_upload_rows(E, tok, pos, slot, n) : tc_upload_rows(E, tok, pos, slot, n);
+}
+
 // Position-range splits of decode attention (each range >= 1024 positions); one formula for the
 // step and for its graph-cache key.  (Also limiting the splits by rows x kv heads measured the
 // same at 256 rows.)
@@ -1017,10 +1144,28 @@ static bool tc_step(Engine* E, int n, int lrow0, int nlog, int max_pos, int pref
     const size_t qkv_stride = (size_t)E->tc_T * (dim + 2 * kvd);
     const int sq = tc_launch(E, Y.qkv, E->img_d, n, -1,
                              rows(E->t_qkv, dim + 2 * kvd, dim + 2 * kvd, qkv_stride));
-    if (prefill_p0 >= 0 || !fold)
+    if (E->paged) {
+      const llama_paged_kv_t kv = paged_desc(E, n, l);
+      const int32_t* seq = E->t_idx + 3 * n;
+      const int32_t* cu = E->t_idx + 4 * n;
+      paged::Waits waits;
+      waits.error = E->tc_err;
+      waits.ns = E->attn_wait_ns;
+      waits.expire = E->attn_expire;
+      const char* why = paged::append_rows(&kv, E->t_qkv, LLAMA_F32, dim + 2 * kvd, sq, (int64_t)qkv_stride, n,
+                                           (int)E->heads, pos, seq, E->rope_cos, E->rope_sin, LE_MAX_SEQ_LEN, E->t_q,
+                                           E->page_type, dim, s, true);
+      if (!why)
+        why = paged::attention_rows(&kv, E->device, E->t_q, dim, (int)E->heads, cu, cu + E->runs + 1, n, E->run_q,
+                                    E->run_kv, 0.125f, E->t_attn, LLAMA_F32, dim, E->paged_ws, waits, s, true);
+      if (why) { E->err = std::string("paged attention: ") + why; return false; }
+    } else if (prefill_p0 >= 0 || !fold) {
       launch_pdl(k_rope_append, dim3(n), dim3(256), 0, s, E->t_qkv, sq, qkv_stride,
                  dim, kvd, pos, slot, E->rope_cos, E->rope_sin, E->t_q, kc, vc, slot_stride);
-    if (prefill_p0 >= 0) {
+    }
+    if (E->paged) {
+      // attended above
+    } else if (prefill_p0 >= 0) {
       const int p_last = prefill_p0 + n - 1;
       launch_pdl(k_kv_tiles, dim3(E->kv_heads, p_last / attn::kKeys + 1), dim3(128), 0, s, kc, vc, kvd, p_last,
                  E->kv_img, E->kv_img_tiles);
@@ -1037,7 +1182,7 @@ static bool tc_step(Engine* E, int n, int lrow0, int nlog, int max_pos, int pref
         launch_pdl(k_attn_combine, dim3(n), dim3(256), 0, s, E->t_attn_part, (int)E->kv_heads, attn_splits, dim,
                    E->t_attn);
     }
-    if (prefill_p0 >= 0 || attn_splits > 1)
+    if (prefill_p0 >= 0 || attn_splits > 1 || E->paged)
       launch_pdl(stage_fn, dim3(n, dim / 2048), dim3(256), 0, s, E->t_attn, dim, nullptr, 0, 0, nullptr, dim,
                  E->img_d);
     const int so = tc_launch(E, Y.o, E->img_d, n, -1, rows(E->t_part, dim, dim, part_stride));
@@ -1069,7 +1214,8 @@ static bool tc_step(Engine* E, int n, int lrow0, int nlog, int max_pos, int pref
 static bool tc_step_graph(Engine* E, int n, int nlog, int max_pos, bool fold) {
   const int splits = attn_splits_for(max_pos);
   for (const auto& g : E->tc_graphs)
-    if (g.n == n && g.nlog == nlog && g.splits == splits && g.fold == fold) {
+    if (g.n == n && g.nlog == nlog && g.splits == splits && g.fold == fold && g.runs == E->runs && g.run_q == E->run_q &&
+        g.run_kv == E->run_kv) {
       LE_CK(cudaGraphLaunch(g.exec, E->stream));
       E->tc_dirty = true;
       return true;
@@ -1088,18 +1234,19 @@ static bool tc_step_graph(Engine* E, int n, int nlog, int max_pos, bool fold) {
   const cudaError_t ie = cudaGraphInstantiate(&exec, graph, 0);
   cudaGraphDestroy(graph);
   if (ie != cudaSuccess) { E->err = cudaGetErrorString(ie); return false; }
-  E->tc_graphs.push_back({n, nlog, splits, fold, exec});
+  E->tc_graphs.push_back({n, nlog, splits, fold, E->runs, E->run_q, E->run_kv, exec});
   LE_CK(cudaGraphLaunch(exec, E->stream));
   return true;
 }
 
 // Chunked prefill of `count` tokens of slot 0 at positions start .. start+count-1.
 static bool tc_prefill(Engine* E, const int32_t* ids, size_t count, size_t start, bool last_logits) {
+  if (!pages_fit(E, start, count)) return false;
   std::vector<int32_t> pos(E->tc_T), slot(E->tc_T, 0);
   for (size_t c0 = 0; c0 < count; c0 += (size_t)E->tc_T) {
     const int n = (int)std::min<size_t>((size_t)E->tc_T, count - c0);
     for (int i = 0; i < n; ++i) pos[i] = (int32_t)(start + c0 + i);
-    if (!tc_upload_rows(E, ids + c0, pos.data(), slot.data(), n)) return false;
+    if (!upload_rows(E, ids + c0, pos.data(), slot.data(), n)) return false;
     const bool lg = last_logits && c0 + n == count;
     if (!tc_step(E, n, n - 1, lg ? 1 : 0, (int)(start + c0) + n - 1, (int)(start + c0))) return false;
   }
@@ -1134,6 +1281,7 @@ static bool check_status(Engine* E) {
   }
   if (tc_read && E->h_err[2] != 0) {
     E->err = (E->h_err[2] == (uint32_t)kExpireAttn ? "prefill attention (tensor cores): a wait timed out (code "
+              : E->h_err[2] == paged::kChunkError  ? "paged attention (tensor cores): a wait timed out (code "
                                                     : "tensor-core GEMM: a pipeline wait timed out (code ") +
              std::to_string(E->h_err[2]) + ")";
     E->tc_dirty = true;  // keep reporting it
@@ -1257,11 +1405,23 @@ static bool init_device(Engine* E, const uint8_t* base, const ParsedFile& P) {
   }
 
   // ---- KV caches and activations ----
-  const size_t kv_elems = (size_t)E->max_batch * E->layers * E->max_seq * E->kv_dim;
-  LE_CK(cudaMalloc(&E->kcache, kv_elems * 4));
-  LE_CK(cudaMalloc(&E->vcache, kv_elems * 4));
-  LE_CK(cudaMemsetAsync(E->kcache, 0, kv_elems * 4, E->stream));
-  LE_CK(cudaMemsetAsync(E->vcache, 0, kv_elems * 4, E->stream));
+  if (E->paged) {
+    const size_t pool = (size_t)E->layers * E->num_pages * E->page_size * E->kv_dim * 2;
+    LE_CK(cudaMalloc(&E->pool_k, pool));
+    LE_CK(cudaMalloc(&E->pool_v, pool));
+    E->page_width = (E->max_seq + E->page_size - 1) / E->page_size;
+    const size_t entries = (size_t)E->max_batch * E->page_width;
+    LE_CK(cudaMalloc(&E->d_table, entries * 4));
+    LE_CK(cudaMemsetAsync(E->d_table, 0xff, entries * 4, E->stream));
+    E->h_table.assign(entries, -1);
+    for (int i = E->num_pages - 1; i >= 0; --i) E->free_pages.push_back(i);
+  } else {
+    const size_t kv_elems = (size_t)E->max_batch * E->layers * E->max_seq * E->kv_dim;
+    LE_CK(cudaMalloc(&E->kcache, kv_elems * 4));
+    LE_CK(cudaMalloc(&E->vcache, kv_elems * 4));
+    LE_CK(cudaMemsetAsync(E->kcache, 0, kv_elems * 4, E->stream));
+    LE_CK(cudaMemsetAsync(E->vcache, 0, kv_elems * 4, E->stream));
+  }
   const size_t B = (size_t)E->max_batch;
   E->lm_grid = std::min<int>((int)((E->vocab / 2 + kWarps - 1) / kWarps), E->num_sms * 8);
   LE_CK(cudaMalloc(&E->x, B * E->dim * 4));
@@ -1296,8 +1456,15 @@ static bool init_device(Engine* E, const uint8_t* base, const ParsedFile& P) {
   if (!capture(E, row_buffers(E, 0, 0, true, 1), &E->g_gen)) return false;
   LE_CK(cudaStreamSynchronize(E->stream));
   if (E->tp_world > 1) return true;  // the tensor-parallel engine runs its own graph (init_tp)
-  if (!init_persistent(E)) return false;
+  if (!E->paged && !init_persistent(E)) return false;
   if (!init_tc(E)) return false;
+  if (E->paged) {
+    if (!E->tc) {
+      if (E->err.empty()) E->err = "a paged engine needs the tensor-core batched path";
+      return false;
+    }
+    LE_CK(cudaMalloc(&E->paged_ws, paged::attention_bytes_max(LE_HEAD_DIM)));
+  }
   return true;
 }
 
@@ -1317,9 +1484,11 @@ static void destroy(Engine* E) {
   if (E->h_done) cudaFreeHost(E->h_done);
   void* tdev[] = {E->tc_arena, E->img_d, E->img_f, E->t_x, E->t_q, E->t_attn, E->t_qkv, E->t_gu, E->t_part,
                   E->t_idx, E->t_am, E->tc_err, E->t_attn_part, E->kv_img, E->sc_logits, E->sc_target, E->sc_lp,
-                  E->sc_greedy};
+                  E->sc_greedy,
+                  E->pool_k, E->pool_v, E->d_table, E->paged_ws, E->d_sample};
   for (void* p : tdev) if (p) cudaFree(p);
   if (E->h_idx) cudaFreeHost(E->h_idx);
+  if (E->h_sample) cudaFreeHost(E->h_sample);
   if (E->idx_ev) cudaEventDestroy(E->idx_ev);
   void* dev_ptrs[] = {E->arena, E->rope_cos, E->rope_sin, E->kcache, E->vcache, E->x, E->qkv, E->attn,
                       E->act, E->logits, E->emb, E->red, E->d_misc, E->part, E->ctrl_block, E->token_log, E->d_params};
@@ -1332,8 +1501,9 @@ static void destroy(Engine* E) {
 }
 
 static bool init_tp(Engine* E, const ncclUniqueId& id);
+struct PagedSpec { int pages, page_size, type; };
 static Engine* create(const char* path, int device, int max_batch, int max_seq, int tp_rank = 0, int tp_world = 1,
-                      const ncclUniqueId* tp_id = nullptr) {
+                      const ncclUniqueId* tp_id = nullptr, const PagedSpec* paged_spec = nullptr) {
   if (!path) { set_create_error("model path is NULL"); return nullptr; }
   if (max_batch < 1 || max_batch > 4096) { set_create_error("max_batch out of range"); return nullptr; }
   if (max_seq == 0) max_seq = LE_MAX_SEQ_LEN;
@@ -1356,6 +1526,12 @@ static Engine* create(const char* path, int device, int max_batch, int max_seq, 
   E->max_seq = max_seq;
   E->tp_rank = tp_rank;
   E->tp_world = tp_world;
+  if (paged_spec) {
+    E->paged = true;
+    E->num_pages = paged_spec->pages;
+    E->page_size = paged_spec->page_size;
+    E->page_type = paged_spec->type;
+  }
   bool good;
   {
     DeviceGuard dg(device);
@@ -1612,7 +1788,12 @@ static bool queue_params(Engine* E, int32_t token, int32_t pos) {
 static bool forward_token(Engine* E, int32_t token, size_t pos, bool logits) {
   if (pos >= (size_t)E->max_seq) return true;  // silent no-op, src/llama_engine.cpp:936
   if (token < 0 || token >= (int32_t)E->vocab) token = 0;  // :937
-  if (E->persist) {
+  if (E->paged) {  // a batched step of one row
+    const int32_t p = (int32_t)pos, slot = 0;
+    E->last_pos = p;
+    if (!paged_upload_rows(E, &token, &p, &slot, 1)) return false;
+    if (!tc_step_graph(E, 1, logits ? 1 : 0, p, true)) return false;
+  } else if (E->persist) {
     E->last_pos = (int32_t)pos;
     if (!launch_persistent(E, 1, logits, token, (int32_t)pos)) return false;
   } else {
@@ -1856,6 +2037,40 @@ LE_API llama_engine_t llama_engine_create_ex(const char* model_path, int device,
   return create(model_path, device, max_batch, max_seq_len);
 }
 
+LE_API llama_engine_t llama_engine_create_paged(const char* model_path, int device, int max_batch, int max_seq_len,
+                                                int num_pages, int page_size, int cache_type) {
+  if (num_pages < 1 || page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0 ||
+      (cache_type != LLAMA_F16 && cache_type != LLAMA_BF16)) {
+    set_create_error("create_paged: needs num_pages >= 1, page_size 16, 32, 64, 128 or 256, and LLAMA_F16 or LLAMA_BF16");
+    return nullptr;
+  }
+  const PagedSpec spec{num_pages, page_size, cache_type};
+  return create(model_path, device, max_batch, max_seq_len, 0, 1, nullptr, &spec);
+}
+
+LE_API int llama_engine_release_slot(llama_engine_t engine, int slot) {
+  if (!engine) return -1;
+  Engine* E = H(engine);
+  if (!E->paged) { E->err = "release_slot: not a paged engine"; return -1; }
+  if (slot < 0 || slot >= E->max_batch) { E->err = "release_slot: slot out of range"; return -1; }
+  DeviceGuard dg(E->device);
+  // stream-ordered: steps already queued keep their pages until they have run
+  if (cudaMemsetAsync(E->d_table + (size_t)slot * E->page_width, 0xff, (size_t)E->page_width * 4, E->stream) != cudaSuccess) {
+    E->err = "release_slot: device error";
+    return -1;
+  }
+  for (int i = 0; i < E->page_width; ++i) {
+    int32_t& e = E->h_table[(size_t)slot * E->page_width + i];
+    if (e >= 0) E->free_pages.push_back(e);
+    e = -1;
+  }
+  return 0;
+}
+
+LE_API int llama_engine_free_pages(llama_engine_t engine) {
+  return engine && H(engine)->paged ? (int)H(engine)->free_pages.size() : -1;
+}
+
 LE_API const char* llama_engine_last_error(llama_engine_t engine) {
   if (engine) return H(engine)->err.c_str();
   std::lock_guard<std::mutex> lk(g_err_mu);
@@ -1872,6 +2087,14 @@ LE_API int llama_engine_generate_greedy(llama_engine_t engine, int32_t first_tok
   if (start_pos + (size_t)n_steps > (size_t)E->max_seq) { E->err = "generate_greedy: positions exceed max_seq_len"; return -1; }
   DeviceGuard dg(E->device);
   if (first_token < 0 || first_token >= (int32_t)E->vocab) first_token = 0;
+  if (E->paged) {  // token by token through the batched path
+    if (!pages_fit(E, start_pos, (size_t)n_steps)) return -1;
+    for (int32_t i = 0; i < n_steps; ++i) {
+      if (!forward_token(E, i ? out_tokens[i - 1] : first_token, start_pos + (size_t)i, true)) return -1;
+      if (!greedy(E, &out_tokens[i])) return -1;
+    }
+    return 0;
+  }
   if (!queue_params(E, first_token, (int32_t)start_pos)) return -1;
   E->last_pos = (int32_t)(start_pos + n_steps - 1);
   if (E->tp_world > 1) {
@@ -1920,7 +2143,7 @@ LE_API int llama_engine_forward_batch(llama_engine_t engine, const int32_t* toke
   }
   DeviceGuard dg(E->device);
   if (E->tc) {
-    if (!tc_upload_rows(E, tokens, positions, slots, n)) return -1;
+    if (!upload_rows(E, tokens, positions, slots, n)) return -1;
     // stream-ordered: a device error (the GEMM's bounded waits) is reported by the next call
     // that synchronises (argmax_batch, get_logits_batch, get_logits, sample)
     // RoPE / KV append inside attention only when no slot repeats (a row may read the k / v
@@ -2101,6 +2324,7 @@ LE_API void* llama_engine_get_stream(llama_engine_t engine) { return engine ? (v
 LE_API int llama_engine_profile_phase(llama_engine_t engine, const char* phase, int iters, float* avg_ms) {
   if (!engine || !phase || iters < 1 || !avg_ms) return -1;
   Engine* E = H(engine);
+  if (E->paged) { E->err = "profile_phase: not available on a paged engine"; return -1; }
   static const char* names[] = {"qkv", "attn", "oproj", "gateup", "down", "lmhead"};
   int ph = -1;
   for (int i = 0; i < 6; ++i)
@@ -2148,6 +2372,40 @@ LE_API int llama_engine_argmax_batch(llama_engine_t engine, int32_t* out_tokens,
   return sync_ok(E) ? 0 : -1;  // reports a device error of the step
 }
 
+LE_API int llama_engine_sample_batch(llama_engine_t engine, const float* temperature, const int32_t* top_k,
+                                     const float* top_p, const float* min_p, const float* uniform, int n,
+                                     int32_t* out_tokens) {
+  if (!engine || !uniform || !out_tokens || n < 1) return -1;
+  Engine* E = H(engine);
+  if (n > E->max_batch) { E->err = "sample_batch: n exceeds max_batch"; return -1; }
+  if (E->vocab > 262144) { E->err = "sample_batch: vocabulary too large"; return -1; }
+  if (E->tp_world > 1) { E->err = "sample_batch: not available on a tensor-parallel engine"; return -1; }
+  DeviceGuard dg(E->device);
+  const size_t row = (size_t)E->max_batch;
+  if ((!E->d_sample && cudaMalloc(&E->d_sample, 6 * row * 4) != cudaSuccess) ||
+      (!E->h_sample && cudaMallocHost(&E->h_sample, 6 * row * 4) != cudaSuccess)) {
+    E->err = "sample_batch: out of memory";
+    return -1;
+  }
+  // parameters in one copy: temperature | top_k | top_p | min_p | uniform, then the ids (the previous
+  // call has waited for its own, so the staging is free)
+  const void* src[5] = {temperature, top_k, top_p, min_p, uniform};
+  for (int i = 0; i < 5; ++i)
+    if (src[i]) std::memcpy(E->h_sample + i * row, src[i], (size_t)n * 4);
+  auto dev = [&](int i) { return src[i] ? static_cast<void*>(E->d_sample + i * row) : nullptr; };
+  cudaError_t e = cudaMemcpyAsync(E->d_sample, E->h_sample, 5 * row * 4, cudaMemcpyHostToDevice, E->stream);
+  if (e == cudaSuccess)
+    e = sampling::sample_rows(E->logits, LLAMA_F32, E->vocab, n, (int)E->vocab, static_cast<float*>(dev(0)),
+                              static_cast<int32_t*>(dev(1)), static_cast<float*>(dev(2)), static_cast<float*>(dev(3)),
+                              static_cast<float*>(dev(4)), E->d_sample + 5 * row, E->device, E->stream);
+  if (e == cudaSuccess)
+    e = cudaMemcpyAsync(E->h_sample + 5 * row, E->d_sample + 5 * row, (size_t)n * 4, cudaMemcpyDeviceToHost, E->stream);
+  if (e != cudaSuccess) { E->err = std::string("sample_batch: ") + cudaGetErrorString(e); return -1; }
+  if (!sync_ok(E)) return -1;  // reports a device error of the step
+  std::memcpy(out_tokens, E->h_sample + 5 * row, (size_t)n * 4);
+  return 0;
+}
+
 LE_API const float* llama_engine_get_logits_batch(llama_engine_t engine, int row) {
   if (!engine) return nullptr;
   Engine* E = H(engine);
@@ -2182,6 +2440,7 @@ LE_API int llama_engine_score_tokens(llama_engine_t engine, const int32_t* token
   Engine* E = H(engine);
   if (start_pos + n > (size_t)E->max_seq) { E->err = "score_tokens: positions exceed max_seq_len"; return -1; }
   DeviceGuard dg(E->device);
+  if (!pages_fit(E, start_pos, n)) return -1;
   if (!score_alloc(E)) return -1;
   std::vector<int32_t> ids(n), pos(n), slot(n, 0), tgt(kScoreRows);
   for (size_t i = 0; i < n; ++i) {
@@ -2192,7 +2451,7 @@ LE_API int llama_engine_score_tokens(llama_engine_t engine, const int32_t* token
   for (size_t c0 = 0; c0 < n; c0 += (size_t)chunk) {
     const int m = (int)std::min<size_t>((size_t)chunk, n - c0);
     if (E->tc) {
-      if (!tc_upload_rows(E, ids.data() + c0, pos.data() + c0, slot.data(), m)) return -1;
+      if (!upload_rows(E, ids.data() + c0, pos.data() + c0, slot.data(), m)) return -1;
       if (!tc_step(E, m, 0, m, pos[c0 + m - 1], pos[c0], E->sc_logits)) return -1;
     } else {
       if (!forward_token(E, ids[c0], (size_t)pos[c0], true)) return -1;

@@ -52,4 +52,34 @@ inline bool allow_smem(F* fn, int bytes, int dev) {
   return d;
 }
 
+// Launchers of the paged-cache operators for checked arguments (paged_ops.cu); nullptr, or why they
+// failed.  chained: the launches may start while the kernel before them runs out (they wait for
+// its results themselves).
+namespace paged {
+constexpr uint32_t kChunkError = 30;  // error word of a wait of the chunk form that ran out
+// The chunk form's bounded waits: where it reports, the bound, and (test only) whether its product
+// issuer first waits on a barrier phase that nothing completes.
+struct Waits {
+  uint32_t* error = nullptr;
+  unsigned long long ns = 2000000000ull;
+  int expire = 0;
+};
+const char* append_rows(const llama_paged_kv_t* kv, const void* qkv, int type, int64_t ld, int planes,
+                        int64_t plane_stride, int rows, int heads, const int32_t* pos, const int32_t* seq,
+                        const float* rope_cos, const float* rope_sin, int n_pos, void* q_out, int q_type, int64_t q_ld,
+                        cudaStream_t st, bool chained);
+size_t attention_bytes_max(int head_dim);  // workspace that covers every call with seqs <= rows
+const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, int64_t q_ld, int heads,
+                           const int32_t* cu_q, const int32_t* kv_len, int rows, int max_q, int max_kv, float scale,
+                           void* out, int out_type, int64_t out_ld, void* workspace, const Waits& waits, cudaStream_t st,
+                           bool chained);
+}  // namespace paged
+
+// llama_sample_rows for checked arguments (sample_ops.cu).
+namespace sampling {
+cudaError_t sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
+                        const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
+                        int32_t* out_ids, int dev, cudaStream_t st);
+}  // namespace sampling
+
 }  // namespace le

@@ -23,8 +23,9 @@ struct Cache {
   void* k;
   void* v;
   const int32_t* table;
+  const int32_t* slots;  // row of the table of each sequence, or nullptr: the sequence's own number
   int64_t page_stride, row_stride, head_stride;  // elements
-  int table_stride, table_width, seqs, num_pages, page_log2, kv_heads;
+  int table_stride, table_width, table_rows, seqs, num_pages, page_log2, kv_heads;
 };
 
 template <typename T> __device__ __forceinline__ float to_f32(T x);
@@ -64,13 +65,20 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   }
 }
 
-// Row of key j of sequence s in the pools (element offset of kv head g), or -1 when the table
-// holds no valid page for it.
-__device__ __forceinline__ int64_t key_offset(const Cache& C, int s, int j, int g) {
-  const int i = j >> C.page_log2;
-  if (i >= C.table_width) return -1;
-  const int page = C.table[(int64_t)s * C.table_stride + i];
-  if (page < 0 || page >= C.num_pages) return -1;
+// The page ids of sequence s (nullptr: a slot outside the table, whose keys do not exist).
+__device__ __forceinline__ const int32_t* pages_of(const Cache& C, int s) {
+  const int row = C.slots ? C.slots[s] : s;
+  return row >= 0 && row < C.table_rows ? C.table + (int64_t)row * C.table_stride : nullptr;
+}
+// Page of entry e, or -1 where there is none.
+__device__ __forceinline__ int page_at(const Cache& C, const int32_t* pages, int e) {
+  const int p = pages && e < C.table_width ? pages[e] : -1;
+  return p < C.num_pages ? p : -1;
+}
+// Row of key j in the pools (element offset of kv head g), or -1.
+__device__ __forceinline__ int64_t key_offset(const Cache& C, const int32_t* pages, int j, int g) {
+  const int page = page_at(C, pages, j >> C.page_log2);
+  if (page < 0) return -1;
   return (int64_t)page * C.page_stride + (int64_t)(j & ((1 << C.page_log2) - 1)) * C.row_stride +
          (int64_t)g * C.head_stride;
 }
@@ -123,13 +131,17 @@ __device__ __forceinline__ void write_part(float* part, int64_t index, int d, fl
   if (d == 0) *reinterpret_cast<float2*>(p + D) = make_float2(m, l);
 }
 
-// out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the splits of a (row, head), M = max m_z.
-// D / 8 threads per (row, head); rows whose sequence has one split were written already.
-// splits / per: [0] sequences of at most small_rows query rows per kv head, [1] the others.
+// How the keys are split and where the parts lie.  [0]: sequences of at most small_rows query rows
+// per kv head, their parts by (sequence, kv head, row of the tile); [1]: the others, by (row, head),
+// behind part1 parts of the first kind.
+constexpr int kDecodeRows = 16;  // query rows of a decode tile: G heads x new tokens
 struct SplitPlan {
   int per[2], splits[2], small_rows;
-  int64_t part1;  // first part (index) of the second kind
+  int64_t part1;
 };
+
+// out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the splits of a (row, head), M = max m_z.
+// D / 8 threads per (row, head); rows whose sequence has one split were written already.
 template <typename O, int D>
 __global__ void __launch_bounds__(128)
     k_paged_combine(Cache C, int heads, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ kv_len, int rows,
@@ -149,10 +161,12 @@ __global__ void __launch_bounds__(128)
   if (lo >= C.seqs) return;
   const Span sp = span_of(C, cu_q, kv_len, lo, rows);
   if (t < sp.first) return;
-  const int kind = sp.n * (heads / C.kv_heads) <= P.small_rows ? 0 : 1;
+  const int G = heads / C.kv_heads, kind = sp.n * G <= P.small_rows ? 0 : 1;
   const int S = P.splits[kind], used = splits_of(sp.len, P.per[kind], S);
   if (used <= 1) return;
-  const float* p = part + (rh * S + (kind ? P.part1 : 0)) * (D + 8);
+  const int64_t index = kind ? P.part1 + rh * S
+                             : (((int64_t)lo * C.kv_heads + h / G) * kDecodeRows + (t - sp.first) * G + h % G) * S;
+  const float* p = part + index * (D + 8);
   float M = -INFINITY;
   for (int z = 0; z < used; ++z) M = fmaxf(M, p[(int64_t)z * (D + 8) + D]);
   float L = 0.0f, a[8] = {};

@@ -31,6 +31,7 @@
 
 #include <cuda.h>
 
+#include "ops.h"
 #include "paged.cuh"
 #include "ptx.cuh"
 
@@ -42,8 +43,6 @@ constexpr int kItemRows = 2 * kTileRows;
 constexpr int kTileKeys = 128;
 constexpr int kChunkThreads = 320;
 constexpr int kBlockBytes = kTileKeys * 128;   // one 64-element column block of 128 rows
-constexpr unsigned long long kChunkWaitNs = 2000000000ull;
-constexpr uint32_t kChunkError = 30;           // error word of a wait that ran out
 constexpr float kLazyLog2 = 8.0f;              // growth of a maximum that forces a rescale (log2)
 template <int D> struct ChunkGeo {
   static constexpr int kCols = D / 64;                       // column blocks of a row
@@ -92,22 +91,22 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
 }
 
 // Waits (bounded) for phase `parity`; false after a timeout here or elsewhere in the CTA.
-__device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t* error) {
+__device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, const Waits& W) {
   if (mbar_try(bar, parity)) return true;
   const unsigned long long t0 = gtimer();
   while (!mbar_try_sleep(bar, parity, 20000)) {
     if (*abort) return false;
-    if (gtimer() - t0 > kChunkWaitNs) {
+    if (gtimer() - t0 > W.ns) {
       *abort = 1u;
-      atomicCAS(error, 0u, kChunkError);
+      atomicCAS(W.error, 0u, kChunkError);
       return false;
     }
   }
   return true;
 }
-__device__ __forceinline__ void chunk_drain(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ void chunk_drain(uint32_t bar, uint32_t parity, const Waits& W) {
   const unsigned long long t0 = gtimer();
-  while (!mbar_try_sleep(bar, parity, 20000) && gtimer() - t0 < kChunkWaitNs) {
+  while (!mbar_try_sleep(bar, parity, 20000) && gtimer() - t0 < W.ns) {
   }
 }
 
@@ -119,7 +118,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     k_paged_chunk(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Cache C,
                   const T* __restrict__ q, int64_t q_ld, int heads, const int32_t* __restrict__ cu_q,
                   const int32_t* __restrict__ kv_len, int rows, float scale, int small_rows, int per, int splits,
-                  O* __restrict__ out, int64_t out_ld, float* __restrict__ part, uint32_t* error) {
+                  O* __restrict__ out, int64_t out_ld, float* __restrict__ part, Waits W) {
   using Geo = ChunkGeo<D>;
   constexpr int kSt = Geo::kStages;
   extern __shared__ uint8_t chunk_smem[];
@@ -128,7 +127,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __shared__ volatile uint32_t s_abort;
   __shared__ int s_item[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  grid_dep_launch();
+  grid_dep_wait();
+  grid_dep_launch();  // the decode form of the same call may start: its inputs are complete
   const int G = heads / C.kv_heads;
   const int g = blockIdx.x % C.kv_heads;
   const int z = (blockIdx.x / C.kv_heads) % splits;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   auto tiles_to = [&](int end) { return end > k_lo ? (end - k_lo + kTileKeys - 1) / kTileKeys : 0; };
   const int nk0 = tiles_to(keys_end(0)), nk1 = tiles_to(keys_end(1));
   const int nk = max(nk0, nk1);
-  const int32_t* table = C.table + (int64_t)s * C.table_stride;
+  const int32_t* table = pages_of(C, s);
   const int page_mask = (1 << C.page_log2) - 1;
   const int k_hi = min(sp.len, k_lo + nk * kTileKeys);  // keys that are loaded
 
@@ -208,8 +208,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // are all of the item's pages valid?  (a table that holds bad ids costs a check per tile)
   bool bad = false;
   for (int e = (k_lo >> C.page_log2) + tid; e <= ((k_hi - 1) >> C.page_log2) && k_hi > k_lo; e += kChunkThreads) {
-    const int p = table[e];
-    bad |= p < 0 || p >= C.num_pages;
+    bad |= page_at(C, table, e) < 0;
   }
   // Q rows into the K-major swizzled layout: tile i, column block, 128 rows of 128 bytes; a negative
   // scale is moved into q, so that the maximum of s is that of scale s
@@ -239,18 +238,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const int box = min(1 << C.page_log2, kTileKeys), boxes = kTileKeys / box;
     bool ok = true;
     int fills = 0;
-    auto page_at = [&](int j) {  // this lane's page of tile j
+    auto page_of = [&](int j) {  // this lane's page of tile j; none: behind the pool's last
       const int key = k_lo + j * kTileKeys + lane * box;
-      const int p = lane < boxes && key < k_hi ? table[key >> C.page_log2] : -1;
-      return p >= 0 && p < C.num_pages ? p : C.num_pages;
+      const int p = lane < boxes && key < k_hi ? page_at(C, table, key >> C.page_log2) : -1;
+      return p >= 0 ? p : C.num_pages;
     };
-    int page = page_at(0);
+    int page = page_of(0);
     for (int j = 0; j < nk && ok; ++j) {
-      const int next = j + 1 < nk ? page_at(j + 1) : 0;
+      const int next = j + 1 < nk ? page_of(j + 1) : 0;
       const int row = (k_lo + j * kTileKeys) & page_mask;  // nonzero only where pages exceed a tile
       for (int v = 0; v < 2 && ok; ++v) {
         const int st = fills % kSt;
-        if (fills >= kSt) ok = __all_sync(0xffffffffu, chunk_wait(bar(kSt + st), (uint32_t)(fills / kSt - 1) & 1u, &s_abort, error));
+        if (fills >= kSt) ok = __all_sync(0xffffffffu, chunk_wait(bar(kSt + st), (uint32_t)(fills / kSt - 1) & 1u, &s_abort, W));
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(bar(st), Geo::kStageBytes);
         __syncwarp();
@@ -262,7 +261,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         ++fills;
         if (v == 1 && j == fix_tile) {
-          ok = __all_sync(0xffffffffu, chunk_wait(bar(st), (uint32_t)((fills - 1) / kSt) & 1u, &s_abort, error));
+          ok = __all_sync(0xffffffffu, chunk_wait(bar(st), (uint32_t)((fills - 1) / kSt) & 1u, &s_abort, W));
           const int r0 = sp.len - (k_lo + j * kTileKeys);  // first row behind the length
           for (int i = lane; i < (kTileKeys - r0) * 8 * Geo::kCols; i += 32) {
             const int cb = i / ((kTileKeys - r0) * 8), x = i % ((kTileKeys - r0) * 8);
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       page = next;
     }
     if (s_abort)  // the copies in flight land before the shared memory goes
-      for (int f = max(0, fills - kSt); f < fills; ++f) chunk_drain(bar(f % kSt), (uint32_t)(f / kSt) & 1u);
+      for (int f = max(0, fills - kSt); f < fills; ++f) chunk_drain(bar(f % kSt), (uint32_t)(f / kSt) & 1u, W);
   } else if (warp == 8) {
     // ---- products ----
     if (lane == 0) {
@@ -289,7 +288,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         last = b;
         last_parity = n & 1;
       };
-      auto wait = [&](int b, int n) { return chunk_wait(bar(b), (uint32_t)n & 1u, &s_abort, error); };
+      auto wait = [&](int b, int n) { return chunk_wait(bar(b), (uint32_t)n & 1u, &s_abort, W); };
       // S_i of key tile j, from fill 2 j of the ring
       auto issue_s = [&](int i, int j) {
         const uint32_t a = base + (uint32_t)(i * Geo::kStageBytes), b = stage0 + (uint32_t)((2 * j % kSt) * Geo::kStageBytes);
@@ -303,7 +302,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       };
       auto full = [&](int f) { return wait(f % kSt, f / kSt); };
       auto free_stage = [&](int f) { commit(kSt + f % kSt, f / kSt); };
-      if (nk > 0 && (ok = full(0))) {
+      if (W.expire) ok = wait(kBarO, 0);  // test only: no product has been issued, so the wait runs out
+      if (ok && nk > 0 && (ok = full(0))) {
         tc::tc_fence_after();
         if (nk0 > 0) issue_s(0, 0);
         if (nk1 > 0) issue_s(1, 0);
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (j + 1 < nk) free_stage(2 * j + 2);
         }
       }
-      if (s_abort && last >= 0) chunk_drain(bar(last), (uint32_t)last_parity);
+      if (s_abort && last >= 0) chunk_drain(bar(last), (uint32_t)last_parity, W);
     }
     __syncwarp();
   } else {
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     float m = -INFINITY, l = 0.0f;  // the maximum that O and l are scaled by
     bool ok = true;
     for (int j = 0; j < nki; ++j) {
-      ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarS + i), (uint32_t)j & 1u, &s_abort, error));
+      ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarS + i), (uint32_t)j & 1u, &s_abort, W));
       if (!ok) break;
       tc::tc_fence_after();
       float sv[kTileKeys];
@@ -374,8 +374,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       if (any_bad) {  // bit x: the tile's keys 16 x .. 16 x + 15 have a page
         const int key = key0 + 16 * (lane & 7);
-        const int p = key < sp.len ? table[key >> C.page_log2] : -1;
-        const unsigned live = __ballot_sync(0xffffffffu, p >= 0 && p < C.num_pages);
+        const unsigned live = __ballot_sync(0xffffffffu, key < sp.len && page_at(C, table, key >> C.page_log2) >= 0);
 #pragma unroll
         for (int x = 0; x < kTileKeys; ++x) sv[x] = (live >> (x / 16)) & 1u ? sv[x] : -INFINITY;
       }
@@ -388,7 +387,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         m = grow ? mt : m;
         l *= alpha;
         if (j > 0) {
-          ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarO + i), (uint32_t)(j - 1) & 1u, &s_abort, error));
+          ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarO + i), (uint32_t)(j - 1) & 1u, &s_abort, W));
           if (!ok) break;
           tc::tc_fence_after();
 #pragma unroll
@@ -421,7 +420,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_arrive_n(bar(kBarP + i), 1);
     }
     if (ok && nki > 0) {
-      ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarO + i), (uint32_t)(nki - 1) & 1u, &s_abort, error));
+      ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarO + i), (uint32_t)(nki - 1) & 1u, &s_abort, W));
       tc::tc_fence_after();
     }
     // ---- result: the row's D outputs, or this split's part of them ----

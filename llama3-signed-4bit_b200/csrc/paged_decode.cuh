@@ -33,7 +33,6 @@
 namespace le {
 namespace paged {
 
-constexpr int kDecodeRows = 16;   // query rows of one tile: G heads x new tokens
 constexpr int kSlice = 16;        // keys a warp takes at a time
 constexpr int kDecodeWarps = 4;
 template <int D> struct DecodeGeo {
@@ -67,17 +66,19 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, 
 }
 
 // Grid: seqs x splits x kv_heads, kv heads fastest (their CTAs read neighbouring bytes of the same
-// rows).  per: keys of a split, a multiple of 64; the last split takes all keys behind it.
+// rows).  per: keys of a split, a multiple of 64; the last split takes all keys behind it.  beside:
+// launched while the chunk form of the same call runs, whose inputs are complete.
 template <typename T, typename O, int D>
 __global__ void __launch_bounds__(32 * kDecodeWarps)
     k_paged_decode(Cache C, const T* __restrict__ q, int64_t q_ld, int heads, const int32_t* __restrict__ cu_q,
-                   const int32_t* __restrict__ kv_len, int rows, float scale_log2, int per, int splits,
+                   const int32_t* __restrict__ kv_len, int rows, float scale_log2, int per, int splits, int beside,
                    O* __restrict__ out, int64_t out_ld, float* __restrict__ part) {
   using Geo = DecodeGeo<D>;
   constexpr int kSt = Geo::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_m[kDecodeWarps][kDecodeRows], s_l[kDecodeWarps][kDecodeRows];
   grid_dep_launch();
+  if (!beside) grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = blockIdx.x % C.kv_heads;
   const int z = (blockIdx.x / C.kv_heads) % splits;
@@ -114,15 +115,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
   const int kw = k0 + kSlice * warp;
   const int ns = k1 > kw ? (k1 - kw + 63) / 64 : 0;
   const uint32_t ring = smem_u32(smem) + (uint32_t)(warp * kSt * 2 * Geo::kSliceBytes);
-  const int32_t* table = C.table + (int64_t)s * C.table_stride;
+  const int32_t* table = pages_of(C, s);
   const T* kp = static_cast<const T*>(C.k) + (int64_t)g * C.head_stride;
   const T* vp = static_cast<const T*>(C.v) + (int64_t)g * C.head_stride;
   int pages = -1;  // lane i: page of slice (block of 32) + i
   auto fetch_pages = [&](int i0) {
     const int j = kw + 64 * (i0 + lane);
-    const int e = j >> C.page_log2;
-    const int p = i0 + lane < ns && e < C.table_width ? table[e] : -1;
-    pages = p < C.num_pages ? p : -1;
+    pages = i0 + lane < ns ? page_at(C, table, j >> C.page_log2) : -1;
   };
   auto load = [&](int i) {
     if (i < ns) {
@@ -271,7 +270,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
     }
     const int t = sp.first + r / G, h = g * G + r % G;
     if (used > 1) {
-      write_part<D>(part, ((int64_t)t * heads + h) * splits + z, d, M, L, a);
+      write_part<D>(part, (((int64_t)s * C.kv_heads + g) * kDecodeRows + r) * splits + z, d, M, L, a);
     } else {
       const float inv = L > 0.0f ? 1.0f / L : 0.0f;  // no key: zeros
 #pragma unroll

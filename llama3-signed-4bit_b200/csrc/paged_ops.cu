@@ -23,15 +23,17 @@ namespace paged {
 // Append.  Row t of qkv is q heads | k heads | v heads; with (c, s) the table row of its position,
 // rot(x)_i = x_i c_i - x_{i + D/2} s_i and rot(x)_{i + D/2} = x_i s_i + x_{i + D/2} c_i for
 // i < D/2, in fp32 without contraction (the engine's own rotation), rounded once to the output
-// type.  A thread takes 8 rotation pairs of one head: two 16-byte runs half a head apart.
+// type.  A thread takes 8 rotation pairs of one head: two 16-byte runs half a head apart.  With
+// planes > 1 (the engine's split-K products, fp32) a row is the sum of its planes, in plane order.
 // ---------------------------------------------------------------------------------------------
 template <typename In, typename Kv, typename Q, int D>
 __global__ void __launch_bounds__(256)
-    k_paged_append(Cache C, const In* __restrict__ qkv, int64_t ld, int rows, int heads,
+    k_paged_append(Cache C, const In* __restrict__ qkv, int64_t ld, int planes, int64_t plane_stride, int rows, int heads,
                    const int32_t* __restrict__ pos, const int32_t* __restrict__ seq,
                    const float* __restrict__ rope_cos, const float* __restrict__ rope_sin, int n_pos,
                    Q* __restrict__ q_out, int64_t q_ld) {
   constexpr int kRuns = D / 16;
+  grid_dep_begin();
   const int per_row = (heads + 2 * C.kv_heads) * kRuns;
   const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (item >= (int64_t)rows * per_row) return;
@@ -44,6 +46,16 @@ __global__ void __launch_bounds__(256)
   float a[8], b[8];
   load8(src, a);
   load8(src + D / 2, b);
+  for (int j = 1; j < planes; ++j) {
+    float x[8], y[8];
+    load8(src + j * plane_stride, x);
+    load8(src + j * plane_stride + D / 2, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] += x[i];
+      b[i] += y[i];
+    }
+  }
   if (h < heads + C.kv_heads) {
     float c[8], sn[8];
     load8(rope_cos + (int64_t)p * (D / 2) + i0, c);
@@ -62,7 +74,7 @@ __global__ void __launch_bounds__(256)
     return;
   }
   const bool is_k = h < heads + C.kv_heads;
-  const int64_t off = key_offset(C, s, p, is_k ? h - heads : h - heads - C.kv_heads);
+  const int64_t off = key_offset(C, pages_of(C, s), p, is_k ? h - heads : h - heads - C.kv_heads);
   if (off < 0) return;
   Kv* dst = static_cast<Kv*>(is_k ? C.k : C.v) + off + i0;
   store8(dst, a);
@@ -86,6 +98,7 @@ static const char* check_cache(const llama_paged_kv_t* kv) {
   if (kv->page_size < 16 || kv->page_size > 256 || (kv->page_size & (kv->page_size - 1)) != 0)
     return "page_size must be 16, 32, 64, 128 or 256";
   if (kv->num_pages < 1 || kv->kv_heads < 1 || kv->seqs < 1) return "num_pages, kv_heads and seqs must be positive";
+  if (kv->slots ? kv->table_rows < 1 : kv->table_rows != 0) return "table_rows must be positive with slots, 0 without";
   if (kv->table_width < 1 || kv->table_stride < kv->table_width) return "table_stride must be at least table_width >= 1";
   if (kv->table_width > (1 << 30) / kv->page_size) return "table_width is too large";
   if (!aligned16(kv->k) || !aligned16(kv->v)) return "k and v must be 16-byte aligned";
@@ -105,113 +118,13 @@ static Cache cache_of(const llama_paged_kv_t* kv) {
   c.head_stride = kv->head_stride;
   c.table_stride = kv->table_stride;
   c.table_width = kv->table_width;
+  c.slots = kv->slots;
+  c.table_rows = kv->slots ? kv->table_rows : kv->seqs;
   c.seqs = kv->seqs;
   c.num_pages = kv->num_pages;
   while ((1 << c.page_log2) < kv->page_size) ++c.page_log2;
   c.kv_heads = kv->kv_heads;
   return c;
-}
-
-}  // namespace paged
-}  // namespace le
-
-using namespace le;
-
-LE_API int llama_paged_append(const llama_paged_kv_t* kv, const void* qkv, int type, int64_t ld, int rows, int heads,
-                              const int32_t* pos, const int32_t* seq, const float* rope_cos, const float* rope_sin,
-                              int n_pos, void* q_out, int q_type, int64_t q_ld, void* stream) {
-  using namespace paged;
-  const char* who = "llama_paged_append";
-  if (const char* why = check_cache(kv)) return refuse(who, why);
-  if (!qkv || !pos || !seq || !rope_cos || !rope_sin || !q_out) return refuse(who, "NULL argument");
-  if (type != LLAMA_F32 && type != kv->type) return refuse(who, "type must be LLAMA_F32 or the cache's type");
-  if (q_type != type && q_type != kv->type) return refuse(who, "q_type must be the input's or the cache's type");
-  if (rows < 0 || n_pos < 1) return refuse(who, "rows and n_pos out of range");
-  if (heads < 1 || heads > 4096 || heads % kv->kv_heads != 0) return refuse(who, "heads must be a multiple of kv_heads");
-  const int D = kv->head_dim;
-  if (ld < (int64_t)(heads + 2 * kv->kv_heads) * D || (ld * type_size(type)) % 16 != 0)
-    return refuse(who, "ld is shorter than a row or not a multiple of 16 bytes");
-  if (q_ld < (int64_t)heads * D || (q_ld * type_size(q_type)) % 16 != 0)
-    return refuse(who, "q_ld is shorter than a row or not a multiple of 16 bytes");
-  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(rope_cos) || !aligned16(rope_sin))
-    return refuse(who, "qkv, q_out and the RoPE tables must be 16-byte aligned");
-  if (rows == 0) return 0;
-  const int dev = device_of(kv->k);
-  const void* ptrs[] = {kv->v, kv->table, qkv, pos, seq, rope_cos, rope_sin, q_out};
-  for (const void* p : ptrs)
-    if (dev < 0 || device_of(p) != dev) return refuse(who, "every pointer must be memory of one CUDA device");
-  DeviceGuard dg(dev);
-  const Cache C = cache_of(kv);
-  const int64_t items = (int64_t)rows * (heads + 2 * kv->kv_heads) * (D / 16);
-  if (items > (int64_t)256 * 0x7fffffff) return refuse(who, "rows out of range");
-  const unsigned grid = (unsigned)((items + 255) / 256);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto launch = [&](auto in, auto c, auto q) {
-    using In = decltype(in);
-    using Kv = decltype(c);
-    using Q = decltype(q);
-    auto* fn = D == 64 ? k_paged_append<In, Kv, Q, 64> : k_paged_append<In, Kv, Q, 128>;
-    fn<<<grid, 256, 0, st>>>(C, static_cast<const In*>(qkv), ld, rows, heads, pos, seq, rope_cos, rope_sin, n_pos,
-                             static_cast<Q*>(q_out), q_ld);
-  };
-  auto by_type = [&](auto c) {
-    if (type != LLAMA_F32) launch(c, c, c);
-    else if (q_type == LLAMA_F32) launch(0.0f, c, 0.0f);
-    else launch(0.0f, c, c);
-  };
-  if (kv->type == LLAMA_F16) by_type(__half{});
-  else by_type(__nv_bfloat16{});
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : refuse(who, cudaGetErrorString(e));
-}
-
-namespace le {
-namespace paged {
-
-constexpr int kSms = 148;  // the workspace's size must not need a device
-
-// How a call is cut: which kernels run, and their key splits.
-struct Plan {
-  SplitPlan sp{};
-  bool decode = false, chunk = false;
-  size_t bytes = 0;
-};
-static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, int max_kv) {
-  Plan P;
-  const int G = heads / kv->kv_heads;
-  const int64_t keys = std::max<int64_t>(1, std::min<int64_t>(max_kv, (int64_t)kv->table_width * kv->page_size));
-  P.chunk = (int64_t)max_q * G > kDecodeRows;
-  // beside chunks there are sequences of few tokens unless all have max_q of them
-  P.decode = !P.chunk || (kv->seqs > 1 && rows < (int64_t)kv->seqs * max_q && G <= kDecodeRows);
-  P.sp.small_rows = P.decode ? kDecodeRows : 0;
-  const int64_t units = (int64_t)std::min(kv->seqs, std::max(rows, 1)) * kv->kv_heads;
-  // decode: about eight CTAs for every SM where the keys allow, of 64 keys (one slice for each warp) at least
-  int64_t per = (units * keys + kSms * 8 - 1) / (kSms * 8);
-  per = std::max<int64_t>(64, (per + 63) / 64 * 64);
-  P.sp.per[0] = (int)per;
-  P.sp.splits[0] = P.decode ? (int)((keys + per - 1) / per) : 1;
-  // chunk: one CTA per SM; as many splits as make the estimated waves x (a split's keys + the fixed
-  // cost of an item, about that of 256 keys) smallest, at least 512 keys each
-  P.sp.per[1] = 1 << 30;
-  P.sp.splits[1] = 1;
-  if (P.chunk) {
-    const int64_t items = std::max<int64_t>(1, ((int64_t)rows * G + kItemRows - 1) / kItemRows) * kv->kv_heads;
-    int64_t best = -1;
-    for (int64_t n = 1; n <= 32 && (n == 1 || keys >= 512 * n); ++n) {
-      const int64_t p1 = (keys + n * kTileKeys - 1) / (n * kTileKeys) * kTileKeys;
-      const int64_t cost = (items * n + kSms - 1) / kSms * (p1 + 256);
-      if (best < 0 || cost < best) {
-        best = cost;
-        P.sp.per[1] = n == 1 ? 1 << 30 : (int)p1;
-        P.sp.splits[1] = (int)((keys + p1 - 1) / p1);
-      }
-    }
-  }
-  const int64_t pairs = (int64_t)rows * heads;
-  const int64_t n0 = P.sp.splits[0] > 1 ? pairs * P.sp.splits[0] : 0, n1 = P.sp.splits[1] > 1 ? pairs * P.sp.splits[1] : 0;
-  P.sp.part1 = n0;
-  P.bytes = (size_t)(n0 + n1) * (kv->head_dim + 8) * sizeof(float);
-  return P;
 }
 
 // A launch that may start while the kernel before it runs out; that kernel's results are there
@@ -230,6 +143,81 @@ static void launch(bool early, void (*kernel)(KArgs...), unsigned grid, unsigned
   cfg.attrs = at;
   cfg.numAttrs = early ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+const char* append_rows(const llama_paged_kv_t* kv, const void* qkv, int type, int64_t ld, int planes,
+                        int64_t plane_stride, int rows, int heads, const int32_t* pos, const int32_t* seq,
+                        const float* rope_cos, const float* rope_sin, int n_pos, void* q_out, int q_type, int64_t q_ld,
+                        cudaStream_t st, bool chained) {
+  const Cache C = cache_of(kv);
+  const int D = kv->head_dim;
+  const int64_t items = (int64_t)rows * (heads + 2 * kv->kv_heads) * (D / 16);
+  if (items > (int64_t)256 * 0x7fffffff) return "rows out of range";
+  const unsigned grid = (unsigned)((items + 255) / 256);
+  auto run = [&](auto in, auto c, auto q) {
+    using In = decltype(in);
+    using Kv = decltype(c);
+    using Q = decltype(q);
+    auto* fn = D == 64 ? k_paged_append<In, Kv, Q, 64> : k_paged_append<In, Kv, Q, 128>;
+    launch(chained, fn, grid, 256, 0, st, C, static_cast<const In*>(qkv), ld, planes, plane_stride, rows, heads, pos, seq,
+           rope_cos, rope_sin, n_pos, static_cast<Q*>(q_out), q_ld);
+  };
+  auto by_type = [&](auto c) {
+    if (type != LLAMA_F32) run(c, c, c);
+    else if (q_type == LLAMA_F32) run(0.0f, c, 0.0f);
+    else run(0.0f, c, c);
+  };
+  if (kv->type == LLAMA_F16) by_type(__half{});
+  else by_type(__nv_bfloat16{});
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+}
+
+constexpr int kSms = 148;  // the workspace's size must not need a device
+constexpr int kDecodeCtas = 8 * kSms, kChunkItems = 4 * kSms;  // bounds of what splitting makes
+
+// How a call is cut: which kernels run, and their key splits.
+struct Plan {
+  SplitPlan sp{};
+  bool decode = false, chunk = false;
+  size_t bytes = 0;
+};
+static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, int max_kv) {
+  Plan P;
+  const int G = heads / kv->kv_heads;
+  const int64_t keys = std::max<int64_t>(1, std::min<int64_t>(max_kv, (int64_t)kv->table_width * kv->page_size));
+  P.chunk = (int64_t)max_q * G > kDecodeRows;
+  // beside chunks there are sequences of few tokens unless all have max_q of them
+  P.decode = !P.chunk || (kv->seqs > 1 && rows < (int64_t)kv->seqs * max_q && G <= kDecodeRows);
+  P.sp.small_rows = P.decode ? kDecodeRows : 0;
+  const int64_t units = (int64_t)std::min(kv->seqs, std::max(rows, 1)) * kv->kv_heads;
+  // decode: about eight CTAs for every SM where the keys allow, of 64 keys (one slice for each warp) at least
+  int64_t per = (units * keys + kDecodeCtas - 1) / kDecodeCtas;
+  per = std::max<int64_t>(64, (per + 63) / 64 * 64);
+  P.sp.per[0] = (int)per;
+  P.sp.splits[0] = P.decode ? (int)((keys + per - 1) / per) : 1;
+  // chunk: one CTA per SM; as many splits as make the estimated waves x (a split's keys + the fixed
+  // cost of an item, about that of 256 keys) smallest, at least 512 keys each
+  P.sp.per[1] = 1 << 30;
+  P.sp.splits[1] = 1;
+  if (P.chunk) {
+    const int64_t items = std::max<int64_t>(1, ((int64_t)rows * G + kItemRows - 1) / kItemRows) * kv->kv_heads;
+    int64_t best = -1;
+    for (int64_t n = 1; n == 1 || (n <= 32 && keys >= 512 * n && items * n <= kChunkItems); ++n) {
+      const int64_t p1 = (keys + n * kTileKeys - 1) / (n * kTileKeys) * kTileKeys;
+      const int64_t cost = (items * n + kSms - 1) / kSms * (p1 + 256);
+      if (best < 0 || cost < best) {
+        best = cost;
+        P.sp.per[1] = n == 1 ? 1 << 30 : (int)p1;
+        P.sp.splits[1] = (int)((keys + p1 - 1) / p1);
+      }
+    }
+  }
+  const int64_t n0 = P.sp.splits[0] > 1 ? (int64_t)kv->seqs * kv->kv_heads * kDecodeRows * P.sp.splits[0] : 0;
+  const int64_t n1 = P.sp.splits[1] > 1 ? (int64_t)rows * heads * P.sp.splits[1] : 0;
+  P.sp.part1 = n0;
+  P.bytes = (size_t)(n0 + n1) * (kv->head_dim + 8) * sizeof(float);
+  return P;
 }
 
 // TMA map of a pool: (element, head, row, page), boxes of 64 elements x one head x up to 128 rows of a
@@ -270,7 +258,7 @@ static uint32_t* error_word(int dev) {
 template <typename T, typename O, int D>
 static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Cache& C, int dev, const void* q, int64_t q_ld, int heads,
                              const int32_t* cu_q, const int32_t* kv_len, int rows, float scale, void* out,
-                             int64_t out_ld, float* part, cudaStream_t st) {
+                             int64_t out_ld, float* part, const Waits& waits, cudaStream_t st, bool chained) {
   const T* qt = static_cast<const T*>(q);
   O* ot = static_cast<O*>(out);
   if (P.chunk) {
@@ -279,19 +267,18 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
     const int64_t grid = items * C.kv_heads * P.sp.splits[1];
     if (grid > 0x7fffffff) return "too many rows";
     CUtensorMap mk, mv;
-    uint32_t* err = error_word(dev);
-    if (!err || !pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v)) return "tensor maps of the pools could not be made";
+    if (!pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v)) return "tensor maps of the pools could not be made";
     if (!allow_smem(k_paged_chunk<T, O, D>, ChunkGeo<D>::kSmem, dev)) return "shared memory could not be set";
-    launch(false, k_paged_chunk<T, O, D>, (unsigned)grid, kChunkThreads, ChunkGeo<D>::kSmem, st, mk, mv, C, qt, q_ld, heads,
+    launch(chained, k_paged_chunk<T, O, D>, (unsigned)grid, kChunkThreads, ChunkGeo<D>::kSmem, st, mk, mv, C, qt, q_ld, heads,
            cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], ot, out_ld,
-           part + P.sp.part1 * (D + 8), err);
+           part + P.sp.part1 * (D + 8), waits);
   }
   if (P.decode) {
     const int64_t grid = (int64_t)C.seqs * C.kv_heads * P.sp.splits[0];
     if (grid > 0x7fffffff) return "too many sequences";
     if (!allow_smem(k_paged_decode<T, O, D>, DecodeGeo<D>::kSmem, dev)) return "shared memory could not be set";
-    launch(P.chunk, k_paged_decode<T, O, D>, (unsigned)grid, 32 * kDecodeWarps, DecodeGeo<D>::kSmem, st, C, qt, q_ld,
-           heads, cu_q, kv_len, rows, scale * 1.44269504f, P.sp.per[0], P.sp.splits[0], ot, out_ld, part);
+    launch(P.chunk || chained, k_paged_decode<T, O, D>, (unsigned)grid, 32 * kDecodeWarps, DecodeGeo<D>::kSmem, st, C, qt, q_ld,
+           heads, cu_q, kv_len, rows, scale * 1.44269504f, P.sp.per[0], P.sp.splits[0], P.chunk ? 1 : 0, ot, out_ld, part);
   }
   if (P.sp.splits[0] > 1 || P.sp.splits[1] > 1) {
     const int64_t grid = ((int64_t)rows * heads * (D / 8) + 127) / 128;
@@ -301,8 +288,66 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
   return nullptr;
 }
 
+// No plan for seqs <= rows needs more: a decode tile is split only while there are fewer than
+// kDecodeCtas (sequence, kv head) pairs, into at most kDecodeCtas + that many splits in all; chunks into
+// at most kChunkItems (item, split) pairs of kItemRows rows.
+size_t attention_bytes_max(int head_dim) {
+  return ((size_t)kDecodeRows * 2 * kDecodeCtas + (size_t)kItemRows * kChunkItems) * (head_dim + 8) * sizeof(float);
+}
+
+const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, int64_t q_ld, int heads,
+                           const int32_t* cu_q, const int32_t* kv_len, int rows, int max_q, int max_kv, float scale,
+                           void* out, int out_type, int64_t out_ld, void* workspace, const Waits& waits, cudaStream_t st,
+                           bool chained) {
+  const Plan P = plan_of(kv, heads, rows, max_q, max_kv);
+  const Cache C = cache_of(kv);
+  auto run = [&](auto c, auto o) {
+    using T = decltype(c);
+    using O = decltype(o);
+    auto* fn = kv->head_dim == 64 ? attention<T, O, 64> : attention<T, O, 128>;
+    return fn(kv, P, C, dev, q, q_ld, heads, cu_q, kv_len, rows, scale, out, out_ld, static_cast<float*>(workspace), waits,
+              st, chained);
+  };
+  auto by_type = [&](auto c) { return out_type == LLAMA_F32 ? run(c, 0.0f) : run(c, c); };
+  if (const char* why = kv->type == LLAMA_F16 ? by_type(__half{}) : by_type(__nv_bfloat16{})) return why;
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+}
+
 }  // namespace paged
 }  // namespace le
+
+using namespace le;
+
+LE_API int llama_paged_append(const llama_paged_kv_t* kv, const void* qkv, int type, int64_t ld, int rows, int heads,
+                              const int32_t* pos, const int32_t* seq, const float* rope_cos, const float* rope_sin,
+                              int n_pos, void* q_out, int q_type, int64_t q_ld, void* stream) {
+  using namespace paged;
+  const char* who = "llama_paged_append";
+  if (const char* why = check_cache(kv)) return refuse(who, why);
+  if (!qkv || !pos || !seq || !rope_cos || !rope_sin || !q_out) return refuse(who, "NULL argument");
+  if (type != LLAMA_F32 && type != kv->type) return refuse(who, "type must be LLAMA_F32 or the cache's type");
+  if (q_type != type && q_type != kv->type) return refuse(who, "q_type must be the input's or the cache's type");
+  if (rows < 0 || n_pos < 1) return refuse(who, "rows and n_pos out of range");
+  if (heads < 1 || heads > 4096 || heads % kv->kv_heads != 0) return refuse(who, "heads must be a multiple of kv_heads");
+  const int D = kv->head_dim;
+  if (ld < (int64_t)(heads + 2 * kv->kv_heads) * D || (ld * type_size(type)) % 16 != 0)
+    return refuse(who, "ld is shorter than a row or not a multiple of 16 bytes");
+  if (q_ld < (int64_t)heads * D || (q_ld * type_size(q_type)) % 16 != 0)
+    return refuse(who, "q_ld is shorter than a row or not a multiple of 16 bytes");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(rope_cos) || !aligned16(rope_sin))
+    return refuse(who, "qkv, q_out and the RoPE tables must be 16-byte aligned");
+  if (rows == 0) return 0;
+  const int dev = device_of(kv->k);
+  const void* ptrs[] = {kv->v, kv->table, qkv, pos, seq, rope_cos, rope_sin, q_out, kv->slots};
+  for (const void* p : ptrs)
+    if (dev < 0 || (p && device_of(p) != dev)) return refuse(who, "every pointer must be memory of one CUDA device");
+  DeviceGuard dg(dev);
+  if (const char* why = append_rows(kv, qkv, type, ld, 1, 0, rows, heads, pos, seq, rope_cos, rope_sin, n_pos, q_out, q_type,
+                                    q_ld, static_cast<cudaStream_t>(stream), false))
+    return refuse(who, why);
+  return 0;
+}
 
 LE_API size_t llama_paged_attention_workspace(const llama_paged_kv_t* kv, int heads, int rows, int max_q, int max_kv) {
   using namespace paged;
@@ -332,20 +377,15 @@ LE_API int llama_paged_attention(const llama_paged_kv_t* kv, const void* q, int6
   if (P.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < P.bytes))
     return refuse(who, "workspace is too small", -2);
   const int dev = device_of(kv->k);
-  const void* ptrs[] = {kv->v, kv->table, q, cu_q, kv_len, out, workspace};
+  const void* ptrs[] = {kv->v, kv->table, q, cu_q, kv_len, out, workspace, kv->slots};
   for (const void* p : ptrs)
     if (dev < 0 || (p && device_of(p) != dev)) return refuse(who, "every pointer must be memory of one CUDA device");
   DeviceGuard dg(dev);
-  const Cache C = cache_of(kv);
-  auto run = [&](auto c, auto o) {
-    using T = decltype(c);
-    using O = decltype(o);
-    auto* fn = D == 64 ? attention<T, O, 64> : attention<T, O, 128>;
-    return fn(kv, P, C, dev, q, q_ld, heads, cu_q, kv_len, rows, scale, out, out_ld, static_cast<float*>(workspace),
-              static_cast<cudaStream_t>(stream));
-  };
-  auto by_type = [&](auto c) { return out_type == LLAMA_F32 ? run(c, 0.0f) : run(c, c); };
-  if (const char* why = kv->type == LLAMA_F16 ? by_type(__half{}) : by_type(__nv_bfloat16{})) return refuse(who, why);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : refuse(who, cudaGetErrorString(e));
+  Waits waits;
+  waits.error = error_word(dev);
+  if (!waits.error) return refuse(who, "the device's error word could not be found");
+  if (const char* why = attention_rows(kv, dev, q, q_ld, heads, cu_q, kv_len, rows, max_q, max_kv, scale, out, out_type, out_ld,
+                                       workspace, waits, static_cast<cudaStream_t>(stream), false))
+    return refuse(who, why);
+  return 0;
 }

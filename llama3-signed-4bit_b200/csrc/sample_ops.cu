@@ -375,6 +375,34 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+cudaError_t sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
+                        const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
+                        int32_t* out_ids, int dev, cudaStream_t st) {
+  // eight CTAs share a row
+  const int ranks = kMaxCluster;
+  const int seg = (vocab + ranks - 1) / ranks;
+  auto launch = [&](auto x) {
+    using T = decltype(x);
+    const size_t smem = (size_t)seg * 4;
+    if (!allow_smem(k_sample_rows<T>, (kMaxVocab / kMaxCluster) * 4, dev)) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(rows * ranks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)ranks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_sample_rows<T>, static_cast<const T*>(logits), ld, vocab, seg, temperature, top_k,
+                              top_p, min_p, uniform, out_ids);
+  };
+  const cudaError_t e = type == LLAMA_F32 ? launch(0.0f) : type == LLAMA_F16 ? launch(__half{}) : launch(__nv_bfloat16{});
+  return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
 static int refuse(const char* why, int rc = -1) {
   set_global_error(std::string("llama_sample_rows: ") + why);
   return rc;
@@ -402,29 +430,7 @@ LE_API int llama_sample_rows(const void* logits, int type, int64_t ld, int rows,
   for (const void* p : ptrs)
     if (p && device_of(p) != dev) return refuse("every pointer must be memory of one CUDA device");
   DeviceGuard dg(dev);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // eight CTAs share a row
-  const int ranks = kMaxCluster;
-  const int seg = (vocab + ranks - 1) / ranks;
-  auto launch = [&](auto x) {
-    using T = decltype(x);
-    const size_t smem = (size_t)seg * 4;
-    if (!allow_smem(k_sample_rows<T>, (kMaxVocab / kMaxCluster) * 4, dev)) return cudaErrorInvalidValue;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(rows * ranks));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_sample_rows<T>, static_cast<const T*>(logits), ld, vocab, seg, temperature, top_k,
-                              top_p, min_p, uniform, out_ids);
-  };
-  cudaError_t e = type == LLAMA_F32 ? launch(0.0f) : type == LLAMA_F16 ? launch(__half{}) : launch(__nv_bfloat16{});
-  if (e == cudaSuccess) e = cudaGetLastError();
+  const cudaError_t e = sample_rows(logits, type, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out_ids, dev,
+                                    static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : refuse(cudaGetErrorString(e));
 }

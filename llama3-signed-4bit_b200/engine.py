@@ -31,7 +31,7 @@ class PagedKV(ctypes.Structure):
                 ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
                 ("page_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
                 ("table", _P), ("table_stride", ctypes.c_int32), ("table_width", ctypes.c_int32),
-                ("seqs", ctypes.c_int32)]
+                ("seqs", ctypes.c_int32), ("slots", _P), ("table_rows", ctypes.c_int32)]
 
 
 def ensure_library_built() -> Path:
@@ -125,6 +125,14 @@ class LlamaEngineBindings:
         lib.llama_engine_check_schedule.restype = ctypes.c_int
         lib.llama_engine_debug_waits.argtypes = [_P, ctypes.c_ulonglong, ctypes.c_int]
         lib.llama_engine_debug_waits.restype = ctypes.c_int
+        lib.llama_engine_sample_batch.argtypes = [_P, _FP, _I32P, _FP, _FP, _FP, ctypes.c_int, _I32P]
+        lib.llama_engine_sample_batch.restype = ctypes.c_int
+        lib.llama_engine_create_paged.argtypes = [ctypes.c_char_p] + [ctypes.c_int] * 6
+        lib.llama_engine_create_paged.restype = _P
+        lib.llama_engine_release_slot.argtypes = [_P, ctypes.c_int]
+        lib.llama_engine_release_slot.restype = ctypes.c_int
+        lib.llama_engine_free_pages.argtypes = [_P]
+        lib.llama_engine_free_pages.restype = ctypes.c_int
         i32, i64, kvp = ctypes.c_int, ctypes.c_int64, ctypes.POINTER(PagedKV)
         lib.llama_paged_append.argtypes = [kvp, _P, i32, i64, i32, i32, _P, _P, _P, _P, i32, _P, i32, i64, _P]
         lib.llama_paged_append.restype = ctypes.c_int
@@ -188,18 +196,22 @@ class LlamaEngine:
     """Same surface as the reference's LlamaEngine (src/main.py:188-228), on the GPU.
 
     Extra keyword arguments select the device and the number of independent sequence slots
-    (batched decode); the defaults reproduce ``llama_engine_create``.
+    (batched decode), or a paged KV cache (num_pages > 0); the defaults reproduce
+    ``llama_engine_create``.
     """
 
     def __init__(self, model_path: str, bindings: LlamaEngineBindings, device: int | None = None,
                  max_batch: int = 1, max_seq_len: int = 0, tp_rank: int | None = None, tp_world: int = 1,
-                 tp_unique_id: bytes | None = None):
+                 tp_unique_id: bytes | None = None, num_pages: int = 0, page_size: int = 16, cache_type: int = F16):
         self.bindings = bindings
         lib = bindings.lib
         if tp_rank is not None:  # 2-way tensor-parallel engine (llama_engine_create_tp)
             uid = ctypes.create_string_buffer(tp_unique_id, 128)
             self.handle = lib.llama_engine_create_tp(model_path.encode("utf-8"), device or 0, tp_rank, tp_world,
                                                      uid, max_seq_len)
+        elif num_pages:  # paged 16-bit KV cache shared by the slots (llama_engine_create_paged)
+            self.handle = lib.llama_engine_create_paged(model_path.encode("utf-8"), device or 0, max_batch, max_seq_len,
+                                                        num_pages, page_size, cache_type)
         elif device is None and max_batch == 1 and max_seq_len == 0:
             self.handle = lib.llama_engine_create(model_path.encode("utf-8"))
         else:
@@ -272,6 +284,33 @@ class LlamaEngine:
         out = (ctypes.c_int32 * n)()
         self._check(self.bindings.lib.llama_engine_argmax_batch(self.handle, out, n), "argmax_batch")
         return list(out)
+
+    def sample_batch(self, uniform, temperature=None, top_k=None, top_p=None, min_p=None) -> list[int]:
+        """One id per row of the last forward_batch, drawn on the device from the numbers ``uniform``
+        (in [0, 1)); each rule is None (off), one value for all rows or a value per row."""
+        u = np.ascontiguousarray(uniform, dtype=np.float32).reshape(-1)
+        n = u.size
+
+        def column(x, dtype, ptr):
+            if x is None:
+                return None, None
+            a = np.ascontiguousarray(np.broadcast_to(np.asarray(x, dtype=dtype), (n,)))
+            return a, a.ctypes.data_as(ptr)
+
+        cols = [column(temperature, np.float32, _FP), column(top_k, np.int32, _I32P), column(top_p, np.float32, _FP),
+                column(min_p, np.float32, _FP)]
+        out = (ctypes.c_int32 * max(n, 1))()
+        self._check(self.bindings.lib.llama_engine_sample_batch(self.handle, *[c[1] for c in cols],
+                                                                u.ctypes.data_as(_FP), n, out), "sample_batch")
+        return list(out[:n])
+
+    def release_slot(self, slot: int) -> None:
+        """Returns the slot's pages to the pool (paged engines)."""
+        self._check(self.bindings.lib.llama_engine_release_slot(self.handle, slot), "release_slot")
+
+    @property
+    def free_pages(self) -> int:
+        return self.bindings.lib.llama_engine_free_pages(self.handle)
 
     def get_logits_batch(self, row: int) -> np.ndarray:
         ptr = self.bindings.lib.llama_engine_get_logits_batch(self.handle, row)

@@ -307,6 +307,49 @@ def test_attention_offsets_past_32_bits(pkg, lib):
         check_attention(pool, q, 8, news, lens, out)
 
 
+@pytest.mark.parametrize("news", [[1, 1, 1, 2], [40, 1, 130, 5]])
+def test_sequences_by_slot(pkg, lib, news):
+    """slots names each sequence's row of the table: any order, one row twice, one outside the table
+    (no keys: zeros).  Append and attention agree on it."""
+    import torch
+    cap = [300, 200, 260]
+    pool = Pool(pkg, torch.float16, 4, 64, 32, cap, seed=21)
+    pool.fill(cap)
+    heads, rows = 16, sum(news)
+    slots = torch.tensor([2, 0, 2, 7], dtype=torch.int32, device="cuda")
+    pool.desc.slots, pool.desc.table_rows, pool.desc.seqs = slots.data_ptr(), 3, 4
+    lens = [250, 300, 190, 50]
+    q = torch.randn((rows, heads * 64), device="cuda").half()
+    out = torch.full((rows, heads * 64), 3.0, device="cuda").half()
+    attend(pkg, lib, pool, q, heads, news, lens, out)
+
+    class BySlot:
+        d, kv_heads, dtype = pool.d, pool.kv_heads, pool.dtype
+
+        @staticmethod
+        def rows(s, n):
+            return pool.rows([2, 0, 2][s], n)
+
+    live = rows - news[3]
+    check_attention(BySlot, q, heads, news[:3], lens[:3], out)
+    assert bool((out[live:] == 0).all())
+    # append of one row per sequence at its length
+    cos, sin = rope(64, 512)
+    qkv = torch.randn((4, (heads + 8) * 64), device="cuda")
+    pos = torch.tensor([10, 20, 31, 5], dtype=torch.int32, device="cuda")
+    seq = torch.arange(4, dtype=torch.int32, device="cuda")
+    k0, v0 = pool.k.clone(), pool.v.clone()
+    qo = torch.zeros((4, heads * 64), device="cuda").half()
+    assert lib.llama_paged_append(ctypes.byref(pool.desc), qkv.data_ptr(), pkg.F32, qkv.stride(0), 4, heads, pos.data_ptr(),
+                                  seq.data_ptr(), cos.data_ptr(), sin.data_ptr(), 512, qo.data_ptr(), pkg.F16,
+                                  qo.stride(0), 0) == 0
+    for i, (slot, p) in enumerate([(2, 10), (0, 20), (2, 31)]):
+        pg, sl = pool.where(slot, torch.tensor([p], device="cuda"))
+        assert torch.equal(pool.v[pg, sl].flatten(), qkv[i, (heads + 4) * 64:].half())
+        k0[pg, sl], v0[pg, sl] = pool.k[pg, sl], pool.v[pg, sl]
+    assert torch.equal(k0.nan_to_num(9.0), pool.k.nan_to_num(9.0)) and torch.equal(v0.nan_to_num(9.0), pool.v.nan_to_num(9.0))
+
+
 def test_attention_workspace_is_checked(pkg, lib):
     import torch
     pool = Pool(pkg, torch.float16, 2, 64, 16, [5000], seed=2)

@@ -45,7 +45,8 @@ BAD_CACHES = [dict(k=None), dict(v=None), dict(table=None), dict(type=0), dict(t
               dict(page_size=8), dict(page_size=24), dict(page_size=512), dict(num_pages=0), dict(kv_heads=0),
               dict(seqs=0), dict(table_width=0), dict(table_width=5), dict(k=PTR + 8), dict(v=PTR + 2),
               dict(row_stride=132), dict(head_stride=32), dict(page_stride=-128), dict(page_stride=1 << 40),
-              dict(table_width=1 << 27, table_stride=1 << 27)]
+              dict(table_width=1 << 27, table_stride=1 << 27), dict(slots=PTR), dict(slots=PTR, table_rows=-1),
+              dict(table_rows=3)]
 
 
 @pytest.mark.parametrize("bad", BAD_CACHES, ids=str)
@@ -90,6 +91,13 @@ def test_no_rows_is_no_work(pkg, lib):
     assert append(lib, kv, rows=0) == 0
     assert attend(lib, kv, rows=0) == 0
     assert sample(lib, rows=0) == 0
+
+
+def test_engine_entry_points_refuse_null(lib):
+    assert not lib.llama_engine_create_paged(None, 0, 1, 64, 4, 16, 1)
+    assert lib.llama_engine_release_slot(None, 0) == -1
+    assert lib.llama_engine_free_pages(None) == -1
+    assert lib.llama_engine_sample_batch(None, None, None, None, None, None, 1, None) == -1
 
 
 def test_host_memory_is_refused(pkg, lib):
