@@ -90,6 +90,30 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
       : "memory");
 }
 
+constexpr uint32_t kNegInf = 0xff800000u;
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\t"
+      "mov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // Waits (bounded) for phase `parity`; false after a timeout here or elsewhere in the CTA.
 __device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, const Waits& W) {
   if (mbar_try(bar, parity)) return true;
@@ -351,70 +375,80 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const float c = fmaxf(fabsf(scale) * 1.44269504f, 1e-30f);  // > 0: a masked -inf stays -inf
     const uint32_t t_s = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128u * i;
     const uint32_t t_o = t_s - 128u * i + 256u + 128u * i;
-    float m = -INFINITY, l = 0.0f;  // the maximum that O and l are scaled by
+    float m = -INFINITY, l[2] = {0.0f, 0.0f};  // the maximum that O and l are scaled by; the sum's two halves
     bool ok = true;
     for (int j = 0; j < nki; ++j) {
       ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarS + i), (uint32_t)j & 1u, &s_abort, W));
       if (!ok) break;
       tc::tc_fence_after();
-      float sv[kTileKeys];
-      {
-        uint32_t u[4][32];
+      uint32_t u[4][32];  // the row's 128 scores
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tc::tmem_ld32(t_s + 32u * x, u[x]);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int x = 0; x < kTileKeys; ++x) sv[x] = __uint_as_float(u[x >> 5][x & 31]);
-      }
+      for (int x = 0; x < 4; ++x) tc::tmem_ld32(t_s + 32u * x, u[x]);
+      tc::tmem_wait_ld();
       const int key0 = k_lo + j * kTileKeys;
       if (key0 + kTileKeys - 1 > lim_first) {
         const int rel = lim - key0;
 #pragma unroll
-        for (int x = 0; x < kTileKeys; ++x) sv[x] = x <= rel ? sv[x] : -INFINITY;
+        for (int x = 0; x < kTileKeys; ++x) u[x >> 5][x & 31] = x <= rel ? u[x >> 5][x & 31] : kNegInf;
       }
       if (any_bad) {  // bit x: the tile's keys 16 x .. 16 x + 15 have a page
         const int key = key0 + 16 * (lane & 7);
         const unsigned live = __ballot_sync(0xffffffffu, key < sp.len && page_at(C, table, key >> C.page_log2) >= 0);
 #pragma unroll
-        for (int x = 0; x < kTileKeys; ++x) sv[x] = (live >> (x / 16)) & 1u ? sv[x] : -INFINITY;
+        for (int x = 0; x < kTileKeys; ++x) u[x >> 5][x & 31] = (live >> (x / 16)) & 1u ? u[x >> 5][x & 31] : kNegInf;
       }
-      float mt = fmaxf(sv[0], sv[1]);
+      // maximum, as four chains of three-operand maxima
+      float mx[4];
 #pragma unroll
-      for (int x = 2; x < kTileKeys; ++x) mt = fmaxf(mt, sv[x]);
+      for (int x = 0; x < 4; ++x) {
+        mx[x] = max3(__uint_as_float(u[x][0]), __uint_as_float(u[x][1]), __uint_as_float(u[x][2]));
+#pragma unroll
+        for (int e = 3; e < 31; e += 2) mx[x] = max3(mx[x], __uint_as_float(u[x][e]), __uint_as_float(u[x][e + 1]));
+      }
+      float mt = max3(mx[0], mx[1], mx[2]);
+      mt = max3(mt, mx[3], __uint_as_float(u[0][31]));
+      mt = max3(mt, __uint_as_float(u[1][31]), __uint_as_float(u[2][31]));
+      mt = fmaxf(mt, __uint_as_float(u[3][31]));
       const bool grow = j == 0 ? mt > m : (mt - m) * c > kLazyLog2;
       if (__any_sync(0xffffffffu, grow)) {
         const float alpha = grow ? exp2_approx((m - mt) * c) : 1.0f;
         m = grow ? mt : m;
-        l *= alpha;
+        l[0] *= alpha;
+        l[1] *= alpha;
         if (j > 0) {
           ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarO + i), (uint32_t)(j - 1) & 1u, &s_abort, W));
           if (!ok) break;
           tc::tc_fence_after();
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t v[32];
-            tc::tmem_ld32(t_o + 32u * x, v);
+          for (int x = 0; x < D / 16; ++x) {
+            uint32_t v[16];
+            tc::tmem_ld16(t_o + 16u * x, v);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-            tc::tmem_st32(t_o + 32u * x, v);
+            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+            tmem_st16<16>(t_o + 16u * x, v);
           }
         }
       }
       const float mc = m == -INFINITY ? 0.0f : m * c;
-      float sum = 0.0f;
+      const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
+      float2 sum0 = make_float2(0.0f, 0.0f), sum1 = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float a = exp2_approx(fmaf(sv[32 * x + 2 * e], c, -mc)), b = exp2_approx(fmaf(sv[32 * x + 2 * e + 1], c, -mc));
-          sum += a + b;
-          p[e] = pack2<T>(a, b);
+          float2 y = fma2(make_float2(__uint_as_float(u[x][2 * e]), __uint_as_float(u[x][2 * e + 1])), c2, mc2);
+          y.x = exp2_approx(y.x);
+          y.y = exp2_approx(y.y);
+          if (e & 1) sum1 = add2(sum1, y);
+          else sum0 = add2(sum0, y);
+          p[e] = pack2<T>(y.x, y.y);
         }
         tmem_st16<16>(t_s + 16u * x, p);
       }
-      l += sum;
+      l[0] += sum0.x + sum1.x;
+      l[1] += sum0.y + sum1.y;
       tc::tmem_wait_st();
       tc::tc_fence_before();
       mbar_arrive_n(bar(kBarP + i), 1);
@@ -425,7 +459,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     // ---- result: the row's D outputs, or this split's part of them ----
     const int tok = sp.first + rc / G, h = g * G + rc % G;
-    const float inv = !ok ? NAN : l > 0.0f ? 1.0f / l : 0.0f;
+    const float sum = l[0] + l[1], inv = !ok ? NAN : sum > 0.0f ? 1.0f / sum : 0.0f;
     float* pp = part + (((int64_t)tok * heads + h) * splits + z) * (D + 8);
     O* po = out + (int64_t)tok * out_ld + (int64_t)h * D;
 #pragma unroll
@@ -454,7 +488,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
     }
     if (r < R && used > 1)
-      *reinterpret_cast<float2*>(pp + D) = ok ? make_float2(m == -INFINITY ? m : m * c, l) : make_float2(0.0f, NAN);
+      *reinterpret_cast<float2*>(pp + D) = ok ? make_float2(m == -INFINITY ? m : m * c, sum) : make_float2(0.0f, NAN);
   }
   tc::tc_fence_before();
   __syncthreads();
