@@ -3,30 +3,38 @@
 //
 //   o = sum_j 2^(c s_j - c m) v_j / sum_j 2^(c s_j - c m),  s_j = q . k_j,  c = scale log2(e)
 //
-// The G query heads that share a kv head and the n tokens of a sequence form one axis of n G rows
-// (token-major), cut into work items of 256 rows = two MMA tiles of 128; every key is read once
-// for all 256.  One CTA (one per SM) takes an item and walks its keys in tiles of 128:
+// The G query heads that share a kv head and the n tokens of a sequence form one axis of rows
+// (token-major); a row tile is the 128 / G whole tokens that fit the 128 rows of an MMA (G > 128: 128
+// of a token's heads), and a work item two row tiles of one sequence and kv head, so that every key is
+// read once for up to 256 rows.  One CTA per SM takes items in turn, the longest of each sequence
+// first, and walks an item's keys in tiles of 128:
 //
-//   * warp 9 brings the K and V rows of a tile into a ring of shared-memory stages by TMA, one box
-//     per page and 64-element column block, straight into the 128-byte-swizzled layouts that the
-//     MMA reads: K as the K-major operand of S = Q K^T, V (whose rows are keys) as the MN-major
-//     operand of O += P V, so nothing is transposed.  Pages past the keys, and page ids out of range,
-//     are addressed past the pool's last page: TMA fills them with zeros.  The rows of the last page
-//     behind the length may hold anything, NaN too, which a weight of 0 would not silence: the
-//     loader zeroes them in its V stage and releases that tile's product by a barrier of its own.
+//   * warp 9 finds the items and runs ahead of the others: it publishes an item's description, brings Q
+//     (one box of heads x tokens per column block) and then the K and V rows tile by tile into a ring
+//     of stages by TMA, one box per page and 64-element column block, straight into the
+//     128-byte-swizzled layouts that the MMA reads: K as the K-major operand of S = Q K^T, V (whose
+//     rows are keys) as the MN-major operand of O += P V, so nothing is transposed.  Pages past the
+//     keys, and page ids out of range, are addressed past the pool's last page: TMA fills them with
+//     zeros.  The rows of the last page behind the length may hold anything, NaN too, which a
+//     weight of 0 would not silence: the loader zeroes them in the V stage before it hands it over.
 //   * warp 8 (one thread) issues the products, alternating between the two row tiles so that one
-//     tile's products run while the other's softmax does: P_i V_j, then S_i of the next key tile.
-//     S_i (128 fp32 columns of tensor memory) is overwritten in place by P_i (64 columns), O_i
-//     accumulates in D columns.
+//     tile's products run while the other's softmax does.  S_i is 128 fp32 columns of tensor memory,
+//     P_i 64 columns, O_i head_dim columns.  With head_dim 64 P_i lies beside S_i, and S_i of the
+//     next keys is computed as soon as this one has been read; with 128 P_i replaces S_i.  P is handed
+//     over in two halves, so that the first half's product runs during the second's exponentials.
 //   * warps 0..3 and 4..7 are the softmax of tile 0 and 1, a thread per row (= tensor-memory lane), so
 //     that a row's maximum and sum need no exchange.  O is only rescaled when a row's maximum has
 //     grown by more than 2^8 since the value it is scaled by; until then weights may exceed 1, by at
-//     most 2^8, which costs no accuracy in fp32 sums or 16-bit weights.
+//     most 2^8, which costs no accuracy in fp32 sums or 16-bit weights.  A quarter of the
+//     exponentials is computed on the FMA units (range reduction to
+//     |f| <= 1/2 and a polynomial of degree 5, 1e-7 relative), since 16 a clock and SM is what the
+//     special-function units give.
 // Weights are rounded to the cache's type as the A operand of P V; their sum is taken in fp32 before
-// that.  Bound by the products for head_dim 128 and by the exponentials (16 a clock and SM) for 64.
+// that.
 //
 // All mbarrier waits are bounded; on timeout the error word is set, every role stops, the copies and
-// products in flight are waited for (again bounded) and the item's rows become NaN.
+// products in flight are waited for (again bounded) and the rows of the CTA's remaining items become
+// NaN.
 #pragma once
 
 #include <cuda.h>
@@ -39,17 +47,19 @@ namespace le {
 namespace paged {
 
 constexpr int kTileRows = 128;                 // rows of an MMA tile
-constexpr int kItemRows = 2 * kTileRows;
 constexpr int kTileKeys = 128;
-constexpr int kChunkThreads = 320;
+constexpr int kChunkThreads = 352;             // 2 x 4 softmax warps, products, two loaders
 constexpr int kBlockBytes = kTileKeys * 128;   // one 64-element column block of 128 rows
 constexpr float kLazyLog2 = 8.0f;              // growth of a maximum that forces a rescale (log2)
 template <int D> struct ChunkGeo {
   static constexpr int kCols = D / 64;                       // column blocks of a row
-  static constexpr int kStageBytes = kCols * kBlockBytes;    // K or V of a key tile
+  static constexpr int kStageBytes = kCols * kBlockBytes;    // K or V of a key tile, or Q of a row tile
   static constexpr int kStages = D == 64 ? 8 : 5;
-  static constexpr int kQBytes = 2 * kStageBytes;
-  static constexpr int kSmem = 1024 + kQBytes + kStages * kStageBytes;
+  static constexpr int kQBufs = D == 64 ? 2 : 1;             // items whose Q is held
+  static constexpr int kSmem = 1024 + (2 * kQBufs + kStages) * kStageBytes;
+  // tensor memory (all 512 columns): S_i, P_i and O_i of the two row tiles
+  static constexpr bool kApart = D == 64;                    // P beside S
+  static constexpr uint32_t kColP = kApart ? 256 : 0, kStepP = kApart ? 64 : 128, kColO = 512 - 2 * D;
 };
 
 // Descriptor of a 128-byte-swizzled operand whose 16-bit elements run along N (MN-major): 64-element
@@ -77,6 +87,13 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
           dst),
       "l"(map), "r"(bar), "r"(x), "r"(head), "r"(row), "r"(page)
+      : "memory");
+}
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(map), "r"(bar), "r"(x), "r"(head), "r"(row)
       : "memory");
 }
 template <int N>
@@ -116,379 +133,596 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 
 // Waits (bounded) for phase `parity`; false after a timeout here or elsewhere in the CTA.
 __device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, const Waits& W) {
-  if (mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = gtimer();
-  while (!mbar_try_sleep(bar, parity, 20000)) {
-    if (*abort) return false;
-    if (gtimer() - t0 > W.ns) {
-      *abort = 1u;
-      atomicCAS(W.error, 0u, kChunkError);
-      return false;
+  unsigned long long t0 = 0;
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try(bar, parity)) return true;
+    if ((n & 15u) == 0) {  // now and then: has another thread given up, or the time run out?
+      if (*abort) return false;
+      const unsigned long long t = gtimer();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > W.ns) {
+        *abort = 1u;
+        atomicCAS(W.error, 0u, kChunkError);
+        return false;
+      }
     }
   }
-  return true;
 }
 __device__ __forceinline__ void chunk_drain(uint32_t bar, uint32_t parity, const Waits& W) {
   const unsigned long long t0 = gtimer();
-  while (!mbar_try_sleep(bar, parity, 20000) && gtimer() - t0 < W.ns) {
+  while (!mbar_try(bar, parity) && gtimer() - t0 < W.ns) {
   }
 }
 
-// Grid: items x splits x kv_heads (kv heads fastest), items >= the sum over sequences of
-// ceil(n G / 256); the last items (the longest of each sequence) come first.  per: keys of a split,
-// a multiple of 128.  Sequences of at most small_rows rows per kv head are the decode form's.
+// 2^x for a pair: x = n + f, n the nearest integer, 2^f by a polynomial of degree 5 fitted to the
+// smallest relative error on |f| <= 1/2 (9e-8), n added to the exponent.  x below -126 counts as -126.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 t = add2(x, make_float2(kMagic, kMagic));
+  const float2 n = add2(t, make_float2(-kMagic, -kMagic));
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  float2 p = fma2(make_float2(1.32647292e-3f, 1.32647292e-3f), f, make_float2(9.67151344e-3f, 9.67151344e-3f));
+  p = fma2(p, f, make_float2(5.55073375e-2f, 5.55073375e-2f));
+  p = fma2(p, f, make_float2(2.40222421e-1f, 2.40222421e-1f));
+  p = fma2(p, f, make_float2(6.93146978e-1f, 6.93146978e-1f));
+  p = fma2(p, f, make_float2(1.0f, 1.0f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// How rows are cut into tiles: `tokens` tokens of `heads` heads a tile, `parts` tiles across a token's
+// heads (more than one only for G > 128).
+struct RowTiles {
+  int G, heads, tokens, parts;
+};
+__host__ __device__ __forceinline__ RowTiles row_tiles(int G) {
+  RowTiles t;
+  t.G = G;
+  t.heads = G < kTileRows ? G : kTileRows;
+  t.tokens = kTileRows / t.heads;
+  t.parts = (G + kTileRows - 1) / kTileRows;
+  return t;
+}
+
+// A work item as its CTA's roles see it.
+struct Item {
+  int seq;           // -1: no more
+  int g, z, used;    // kv head, key split, splits of the sequence
+  int first, n, len; // rows and keys of the sequence
+  int unit;          // first of the item's two row tiles
+  int k_lo;          // first key of the split
+  int nk[2];         // key tiles that the row tiles see
+};
+// Item w of the launch (kv heads fastest, then splits, then the row tiles from the last sequence's last),
+// found by a whole warp; the result is the same in every lane.
+__device__ __forceinline__ Item find_item(const Cache& C, const int32_t* cu_q, const int32_t* kv_len, int rows,
+                                          const RowTiles& T, int small_rows, int per, int splits, int total, int w) {
+  const int lane = threadIdx.x & 31;
+  Item it;
+  it.seq = -1;
+  it.g = w % C.kv_heads;
+  it.z = (w / C.kv_heads) % splits;
+  const int want = total - 1 - w / C.kv_heads / splits;
+  int before = 0, local = 0;
+  for (int s0 = 0; s0 < C.seqs && it.seq < 0 && want >= 0; s0 += 32) {
+    int mine = 0;
+    if (s0 + lane < C.seqs) {
+      const int n = max(span_of(C, cu_q, kv_len, s0 + lane, rows).n, 0);
+      mine = n * T.G <= small_rows ? 0 : ((n + T.tokens - 1) / T.tokens * T.parts + 1) / 2;
+    }
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > want);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      it.seq = s0 + l;
+      local = want - before - __shfl_sync(0xffffffffu, inc - mine, l);
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (it.seq < 0) return it;
+  const Span sp = span_of(C, cu_q, kv_len, it.seq, rows);
+  it.first = sp.first;
+  it.n = sp.n;
+  it.len = sp.len;
+  it.unit = 2 * local;
+  it.used = splits_of(sp.len, per, splits);
+  it.k_lo = it.z * per;
+  const int units = (sp.n + T.tokens - 1) / T.tokens * T.parts;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // keys of the tile's rows: all up to its last row's position, within this split
+    const int last = min((it.unit + i) / T.parts * T.tokens + T.tokens, sp.n) - 1;
+    int end = it.unit + i < units && it.z < it.used ? min(sp.len, sp.len - sp.n + last + 1) : 0;
+    if (it.z != splits - 1) end = min(end, it.k_lo + per);
+    it.nk[i] = end > it.k_lo ? (end - it.k_lo + kTileKeys - 1) / kTileKeys : 0;
+  }
+  return it;
+}
+// Row tiles of the whole call, two an item.
+__device__ __forceinline__ int count_items(const Cache& C, const int32_t* cu_q, const int32_t* kv_len, int rows,
+                                           const RowTiles& T, int small_rows) {
+  const int lane = threadIdx.x & 31;
+  int total = 0;
+  for (int s = lane; s < C.seqs; s += 32) {
+    const int n = max(span_of(C, cu_q, kv_len, s, rows).n, 0);
+    if (n * T.G > small_rows) total += ((n + T.tokens - 1) / T.tokens * T.parts + 1) / 2;
+  }
+  return (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+}
+
+// A softmax thread's row of an item.
+struct Row {
+  int tok, h;      // row of q and out, query head
+  int lim;         // last key it sees
+  int lim_first;   // the tile's first row's
+  bool live;       // exists
+};
+__device__ __forceinline__ Row row_of(const Item& it, const RowTiles& T, int i, int r) {
+  Row x;
+  const int unit = it.unit + i, t0 = unit / T.parts * T.tokens, head = unit % T.parts * kTileRows + r % T.heads;
+  const int tok = t0 + r / T.heads, last = min(t0 + T.tokens, it.n) - 1;
+  x.live = r < T.tokens * T.heads && tok < it.n && head < T.G;
+  x.tok = it.first + min(tok, it.n - 1);
+  x.h = it.g * T.G + min(head, T.G - 1);
+  x.lim_first = it.len - it.n + t0;
+  x.lim = it.len - it.n + min(tok, last);  // rows that do not exist see what the last one does
+  return x;
+}
+
+// Grid: one CTA per SM (fewer when there are fewer items).  per: keys of a split, a multiple of 128.
+// Sequences of at most small_rows rows per kv head are the decode form's.
 template <typename T, typename O, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
-    k_paged_chunk(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Cache C,
-                  const T* __restrict__ q, int64_t q_ld, int heads, const int32_t* __restrict__ cu_q,
+    k_paged_chunk(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, Cache C, int heads, const int32_t* __restrict__ cu_q,
                   const int32_t* __restrict__ kv_len, int rows, float scale, int small_rows, int per, int splits,
                   O* __restrict__ out, int64_t out_ld, float* __restrict__ part, Waits W) {
   using Geo = ChunkGeo<D>;
-  constexpr int kSt = Geo::kStages;
+  constexpr int kSt = Geo::kStages, kQb = Geo::kQBufs;
   extern __shared__ uint8_t chunk_smem[];
-  __shared__ __align__(8) unsigned long long s_bar[2 * kSt + 7];
+  // barriers: stage full, stage empty; item published, item read; Q full, Q empty; then per row tile S
+  // ready, S read, P halves, O done, O read; the loader's own for a V tail; one that nothing completes
+  constexpr int kFull = 0, kEmpty = kSt, kItem = 2 * kSt, kItemFree = kItem + 2, kQFull = kItemFree + 2, kQEmpty = kQFull + kQb;
+  constexpr int kBarS = kQEmpty + kQb, kBarR = kBarS + 2, kBarP = kBarR + 2, kBarO = kBarP + 4, kBarE = kBarO + 2;
+  constexpr int kBarFix = kBarE + 2, kNever = kBarFix + 1, kBars = kNever + 1;
+  __shared__ __align__(8) unsigned long long s_bar[kBars];
+  __shared__ Item s_item[2];
   __shared__ uint32_t s_tmem;
   __shared__ volatile uint32_t s_abort;
-  __shared__ int s_item[2];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  grid_dep_wait();
-  grid_dep_launch();  // the decode form of the same call may start: its inputs are complete
-  const int G = heads / C.kv_heads;
-  const int g = blockIdx.x % C.kv_heads;
-  const int z = (blockIdx.x / C.kv_heads) % splits;
-  if (warp == 0) {
-    // the work item: count every sequence's items, then find the one that holds ours from the end
-    auto items_of = [&](int s) {
-      if (s >= C.seqs) return 0;
-      const Span x = span_of(C, cu_q, kv_len, s, rows);
-      const int r = max(x.n, 0) * G;
-      return r <= small_rows ? 0 : (r + kItemRows - 1) / kItemRows;
-    };
-    int total = 0;
-    for (int s0 = 0; s0 < C.seqs; s0 += 32) total += items_of(s0 + lane);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int want = total - 1 - blockIdx.x / C.kv_heads / splits;
-    int before = 0, seq = -1, item = 0;
-    for (int s0 = 0; s0 < C.seqs && seq < 0 && want >= 0; s0 += 32) {
-      const int mine = items_of(s0 + lane);
-      int inc = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > want);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        seq = s0 + l;
-        item = want - before - __shfl_sync(0xffffffffu, inc - mine, l);
-      }
-      before += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    if (lane == 0) {
-      s_item[0] = seq;
-      s_item[1] = item;
-      s_abort = 0u;
-      // full[st] 0.., empty[st] kSt.., S ready (2), P ready (2), O done (2), V tail zeroed
-      for (int i = 0; i < 2 * kSt + 7; ++i) {
-        const bool p = i == 2 * kSt + 2 || i == 2 * kSt + 3;
-        mbar_init(smem_u32(&s_bar[i]), p ? kTileRows : 1);
-      }
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-  }
-  __syncthreads();
-  const int s = s_item[0];
-  const Span sp = s >= 0 ? span_of(C, cu_q, kv_len, s, rows) : Span{0, 0, 0};
-  const int used = splits_of(sp.len, per, splits);
-  if (s < 0 || z >= used) return;  // uniform over the CTA, before any tensor memory is held
-  const int R = sp.n * G;                              // rows of the sequence for this kv head
-  const int row0 = s_item[1] * kItemRows;              // first of this item
-  const int shift = sp.len - sp.n;                     // position of token 0
-  // keys of a tile's rows: all up to its last row's position, within this split
-  const int k_lo = z * per;
-  auto keys_end = [&](int i) {
-    const int r_last = min(row0 + (i + 1) * kTileRows, R) - 1;
-    if (r_last < row0 + i * kTileRows) return 0;
-    const int e = min(sp.len, shift + r_last / G + 1);
-    return z == splits - 1 ? e : min(e, k_lo + per);
-  };
-  auto tiles_to = [&](int end) { return end > k_lo ? (end - k_lo + kTileKeys - 1) / kTileKeys : 0; };
-  const int nk0 = tiles_to(keys_end(0)), nk1 = tiles_to(keys_end(1));
-  const int nk = max(nk0, nk1);
-  const int32_t* table = pages_of(C, s);
-  const int page_mask = (1 << C.page_log2) - 1;
-  const int k_hi = min(sp.len, k_lo + nk * kTileKeys);  // keys that are loaded
-
-  const uint32_t base = (smem_u32(chunk_smem) + 1023u) & ~1023u;
-  const uint32_t stage0 = base + Geo::kQBytes;
+  __shared__ volatile uint32_t s_live[16];  // per key tile: bit x, its keys 16 x .. 16 x + 15 have a page
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   auto bar = [&](int i) { return smem_u32(&s_bar[i]); };
-  const int kBarS = 2 * kSt, kBarP = 2 * kSt + 2, kBarO = 2 * kSt + 4, kBarFix = 2 * kSt + 6;
+  if (tid == 0) {
+    s_abort = 0u;
+    for (int i = 0; i < kBars; ++i) {
+      const bool half = (i >= kBarR && i < kBarO) || (i >= kBarE && i < kBarFix);       // a row tile's threads
+      mbar_init(bar(i), half ? kTileRows : i == kItemFree || i == kItemFree + 1 ? 10 : 1);  // the item's readers
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   if (warp == 8) {
     tc::tmem_alloc(smem_u32(&s_tmem), 512);
     tc::tmem_relinquish();
   }
-  // are all of the item's pages valid?  (a table that holds bad ids costs a check per tile)
-  bool bad = false;
-  for (int e = (k_lo >> C.page_log2) + tid; e <= ((k_hi - 1) >> C.page_log2) && k_hi > k_lo; e += kChunkThreads) {
-    bad |= page_at(C, table, e) < 0;
-  }
-  // Q rows into the K-major swizzled layout: tile i, column block, 128 rows of 128 bytes; a negative
-  // scale is moved into q, so that the maximum of s is that of scale s
-  const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
-  for (int i = tid; i < kItemRows * (D / 8); i += kChunkThreads) {
-    const int r = i / (D / 8), ch = i % (D / 8);
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (row0 + r < R) {
-      const int tok = (row0 + r) / G, h = g * G + (row0 + r) % G;
-      v = *reinterpret_cast<const uint4*>(q + (int64_t)(sp.first + tok) * q_ld + (int64_t)h * D + 8 * ch);
-      v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-    }
-    const uint32_t a = base + (uint32_t)((r >> 7) * Geo::kStageBytes + (ch >> 3) * kBlockBytes + (r & 127) * 128 +
-                                         (((ch & 7) ^ (r & 7)) << 4));
-    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc::tc_fence_before();
-  const bool any_bad = __syncthreads_or(bad ? 1 : 0) != 0;
+  __syncthreads();
   tc::tc_fence_after();
+  grid_dep_wait();
+  grid_dep_launch();  // the decode form of the same call may start: its inputs are complete
   const uint32_t tmem = s_tmem;
-  // a tile that reaches past the length shares its last page with rows that hold anything
-  const int fix_tile = (sp.len & page_mask) != 0 && k_lo + nk * kTileKeys > sp.len ? nk - 1 : -1;
-
-  if (warp == 9) {
-    // ---- loader ----
-    const int box = min(1 << C.page_log2, kTileKeys), boxes = kTileKeys / box;
-    bool ok = true;
-    int fills = 0;
-    auto page_of = [&](int j) {  // this lane's page of tile j; none: behind the pool's last
-      const int key = k_lo + j * kTileKeys + lane * box;
-      const int p = lane < boxes && key < k_hi ? page_at(C, table, key >> C.page_log2) : -1;
-      return p >= 0 ? p : C.num_pages;
-    };
-    int page = page_of(0);
-    for (int j = 0; j < nk && ok; ++j) {
-      const int next = j + 1 < nk ? page_of(j + 1) : 0;
-      const int row = (k_lo + j * kTileKeys) & page_mask;  // nonzero only where pages exceed a tile
-      for (int v = 0; v < 2 && ok; ++v) {
-        const int st = fills % kSt;
-        if (fills >= kSt) ok = __all_sync(0xffffffffu, chunk_wait(bar(kSt + st), (uint32_t)(fills / kSt - 1) & 1u, &s_abort, W));
-        if (!ok) break;
-        if (lane == 0) mbar_expect_tx(bar(st), Geo::kStageBytes);
-        __syncwarp();
-        if (lane < boxes) {
-#pragma unroll
-          for (int cb = 0; cb < Geo::kCols; ++cb)
-            tma_box(stage0 + (uint32_t)(st * Geo::kStageBytes + cb * kBlockBytes + lane * box * 128), v ? &map_v : &map_k,
-                    cb * 64, g, row, page, bar(st));
-        }
-        ++fills;
-        if (v == 1 && j == fix_tile) {
-          ok = __all_sync(0xffffffffu, chunk_wait(bar(st), (uint32_t)((fills - 1) / kSt) & 1u, &s_abort, W));
-          const int r0 = sp.len - (k_lo + j * kTileKeys);  // first row behind the length
-          for (int i = lane; i < (kTileKeys - r0) * 8 * Geo::kCols; i += 32) {
-            const int cb = i / ((kTileKeys - r0) * 8), x = i % ((kTileKeys - r0) * 8);
-            const uint32_t a = stage0 + (uint32_t)(st * Geo::kStageBytes + cb * kBlockBytes + r0 * 128 + x * 16);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0u) : "memory");
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0 && ok) mbar_arrive_n(bar(kBarFix), 1);
-        }
-      }
-      page = next;
-    }
-    if (s_abort)  // the copies in flight land before the shared memory goes
-      for (int f = max(0, fills - kSt); f < fills; ++f) chunk_drain(bar(f % kSt), (uint32_t)(f / kSt) & 1u, W);
-  } else if (warp == 8) {
-    // ---- products ----
-    if (lane == 0) {
-      constexpr uint32_t id_s = chunk_idesc<T>(kTileKeys, 0), id_o = chunk_idesc<T>(D, 1);
+  const RowTiles R = row_tiles(heads / C.kv_heads);
+  const uint32_t base = (smem_u32(chunk_smem) + 1023u) & ~1023u;  // Q buffers of two row tiles, then the stages
+  const uint32_t stage0 = base + (uint32_t)(2 * kQb * Geo::kStageBytes);
+  const int page_mask = (1 << C.page_log2) - 1;
+  if (warp >= 8) {
+    if (warp >= 9) {
+      // ---- loaders: K (and the items and Q), V ----
+      const int kv = warp - 9;
+      const int total = kv == 0 ? count_items(C, cu_q, kv_len, rows, R, small_rows) : 0;
+      const int box = min(1 << C.page_log2, kTileKeys), boxes = kTileKeys / box;
+      const CUtensorMap* const map = kv ? &map_v : &map_k;
+      const bool leader = tc::elect_one();
       bool ok = true;
-      int last = -1, last_parity = 0;
+      int fills = 0, tiles = 0, fixes = 0, qs = 0, last = -1;  // fills: K and V of a tile are two
+      auto wait = [&](int b, int n) { return __all_sync(0xffffffffu, chunk_wait(bar(b), (uint32_t)n & 1u, &s_abort, W)); };
+      for (int w = blockIdx.x, k = 0; ok; w += gridDim.x, ++k) {
+        Item it;
+        if (kv == 0) {
+          it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, w);
+          if (k >= 2) ok = wait(kItemFree + (k & 1), k / 2 - 1);
+          if (!ok) break;
+          if (leader) {
+            s_item[k & 1] = it;
+            mbar_arrive_n(bar(kItem + (k & 1)), 1);
+          }
+        } else {
+          ok = wait(kItem + (k & 1), k / 2);
+          if (!ok) break;
+          it = s_item[k & 1];
+          __syncwarp();
+          if (leader) mbar_arrive_n(bar(kItemFree + (k & 1)), 1);
+        }
+        if (it.seq < 0) break;
+        const int nk = max(it.nk[0], it.nk[1]);
+        if (nk == 0) continue;
+        if (kv == 0) {
+          if (qs >= kQb) ok = wait(kQEmpty + qs % kQb, qs / kQb - 1);
+          if (!ok) break;
+          const int b = qs % kQb, tile_bytes = R.tokens * R.heads * 128 * Geo::kCols;
+          const int both = it.nk[1] > 0 ? 2 : 1;
+          if (leader) {
+            mbar_expect_tx(bar(kQFull + b), (uint32_t)(both * tile_bytes));
+            for (int i = 0; i < both; ++i)
+#pragma unroll
+              for (int cb = 0; cb < Geo::kCols; ++cb)
+                tma_rows(base + (uint32_t)((2 * b + i) * Geo::kStageBytes + cb * kBlockBytes), &map_q, cb * 64,
+                         it.g * R.G + (it.unit + i) % R.parts * kTileRows, it.first + (it.unit + i) / R.parts * R.tokens,
+                         bar(kQFull + b));
+          }
+          __syncwarp();
+          ++qs;
+        }
+        // the key tile that reaches past the length inside a page (the item's last one), if any
+        const int fix = kv && (it.len & page_mask) != 0 && it.k_lo + nk * kTileKeys > it.len ? nk - 1 : -1;
+        const int32_t* table = pages_of(C, it.seq);
+        const int k_hi = min(it.len, it.k_lo + nk * kTileKeys);  // keys that are loaded
+        // this lane's page of tile j as the table has it, loaded a tile ahead and looked at only then;
+        // 0 where no key is wanted
+        auto entry_of = [&](int j) {
+          const int key = it.k_lo + j * kTileKeys + lane * box, e = key >> C.page_log2;
+          return table && lane < boxes && key < k_hi && e < C.table_width ? table[e] : 0;
+        };
+        int entry = entry_of(0);
+        for (int j = 0; j < nk && ok; ++j, ++tiles) {
+          const int next = j + 1 < nk ? entry_of(j + 1) : 0;
+          const int row = (it.k_lo + j * kTileKeys) & page_mask;  // nonzero only where pages exceed a tile
+          const bool wanted = lane < boxes && it.k_lo + j * kTileKeys + lane * box < k_hi;
+          const bool valid = table && entry >= 0 && entry < C.num_pages;
+          const int page = wanted && valid ? entry : C.num_pages;  // none: behind the pool's last
+          const int f = fills + 2 * j + kv, st = f % kSt;
+          if (f >= kSt) ok = wait(kEmpty + st, f / kSt - 1);
+          if (!ok) break;
+          if (kv == 0) {
+            const unsigned gone = __ballot_sync(0xffffffffu, wanted && !valid);
+            uint32_t live = 0xffu;
+            for (int x = 0; gone && x < 8; ++x)
+              if ((gone >> (16 * x / box)) & 1u) live &= ~(1u << x);
+            if (leader) s_live[tiles & 15] = live;
+          }
+          // a stage whose tail is zeroed lands on a barrier of the loader's own first
+          const uint32_t landed = bar(j == fix ? kBarFix : kFull + st);
+          const uint32_t to = stage0 + (uint32_t)(st * Geo::kStageBytes);
+          if (leader) mbar_expect_tx(landed, Geo::kStageBytes);
+          __syncwarp();
+          last = f;
+          // one lane issues the boxes, one after the other: their operands are the warp's
+          auto issue = [&](auto count) {
+            constexpr int n = decltype(count)::value;
+            int pg[n];
+#pragma unroll
+            for (int x = 0; x < n; ++x) pg[x] = __shfl_sync(0xffffffffu, page, x);
+            if (leader) {
+#pragma unroll
+              for (int x = 0; x < n; ++x)
+#pragma unroll
+                for (int cb = 0; cb < Geo::kCols; ++cb)
+                  tma_box(to + (uint32_t)(cb * kBlockBytes + x * (kTileKeys / n) * 128), map, cb * 64, it.g, row, pg[x], landed);
+            }
+          };
+          if (boxes == 8) issue(std::integral_constant<int, 8>{});
+          else if (boxes == 4) issue(std::integral_constant<int, 4>{});
+          else if (boxes == 2) issue(std::integral_constant<int, 2>{});
+          else issue(std::integral_constant<int, 1>{});
+          if (j == fix) {
+            ok = wait(kBarFix, fixes++);
+            const int r0 = it.len - (it.k_lo + j * kTileKeys);  // first row behind the length
+            for (int i = lane; i < (kTileKeys - r0) * 8 * Geo::kCols; i += 32) {
+              const int cb = i / ((kTileKeys - r0) * 8), x = i % ((kTileKeys - r0) * 8);
+              const uint32_t a = to + (uint32_t)(cb * kBlockBytes + r0 * 128 + x * 16);
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0u) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (leader && ok) mbar_arrive_n(bar(kFull + st), 1);
+          }
+          entry = next;
+        }
+        fills += 2 * nk;
+      }
+      if (s_abort) {  // the copies in flight land before the shared memory goes
+        for (int f = last; f >= 0 && f > last - kSt; f -= 2) chunk_drain(bar(kFull + f % kSt), (uint32_t)(f / kSt) & 1u, W);
+        for (int f = max(0, qs - kQb); f < qs; ++f) chunk_drain(bar(kQFull + f % kQb), (uint32_t)(f / kQb) & 1u, W);
+        if (fixes > 0) chunk_drain(bar(kBarFix), (uint32_t)(fixes - 1) & 1u, W);
+      }
+    } else if (warp == 8) {
+      // ---- products ----
+      constexpr uint32_t id_o = chunk_idesc<T>(D, 1);
+      const uint32_t id_s = chunk_idesc<T>(kTileKeys, 0) | (scale < 0.0f ? 1u << 13 : 0u);  // A = -Q: |scale| remains
+      const bool leader = tc::elect_one();
+      bool ok = true;
+      int fills = 0, qs = 0, last = -1, last_parity = 0;
+      int tiles[2] = {0, 0}, reads[2] = {0, 0};  // per row tile: key tiles so far, items that had some
+      auto wait = [&](int b, int n) { return __all_sync(0xffffffffu, chunk_wait(bar(b), (uint32_t)n & 1u, &s_abort, W)); };
       auto commit = [&](int b, int n) {  // n: how often this barrier was committed before
-        tc::tc_commit(bar(b));
+        if (leader) tc::tc_commit(bar(b));
         last = b;
         last_parity = n & 1;
       };
-      auto wait = [&](int b, int n) { return chunk_wait(bar(b), (uint32_t)n & 1u, &s_abort, W); };
-      // S_i of key tile j, from fill 2 j of the ring
-      auto issue_s = [&](int i, int j) {
-        const uint32_t a = base + (uint32_t)(i * Geo::kStageBytes), b = stage0 + (uint32_t)((2 * j % kSt) * Geo::kStageBytes);
+      auto full = [&](int f) { return wait(kFull + f % kSt, f / kSt); };
+      auto free_stage = [&](int f) { commit(kEmpty + f % kSt, f / kSt); };
+      if (W.expire) ok = wait(kNever, 0);  // test only
+      for (int k = 0; ok; ++k) {
+        ok = wait(kItem + (k & 1), k / 2);
+        if (!ok) break;
+        const Item it = s_item[k & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive_n(bar(kItemFree + (k & 1)), 1);
+        if (it.seq < 0) break;
+        const int nk = max(it.nk[0], it.nk[1]);
+        const int q = qs % kQb;
+        // S_i of key tile j; behind it this row tile's count moves on
+        auto issue_s = [&](int i, int j) {
+          const uint32_t a = base + (uint32_t)((2 * q + i) * Geo::kStageBytes);
+          const uint32_t b = stage0 + (uint32_t)((fills + 2 * j) % kSt * Geo::kStageBytes);
+          if (leader) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (uint32_t)((k >> 2) * kBlockBytes);
-          chunk_mma_ss(tmem + 128u * i, tc::sw128_desc(a + off) + 2 * (k & 3), tc::sw128_desc(b + off) + 2 * (k & 3), id_s,
-                       k > 0 ? 1u : 0u);
-        }
-        commit(kBarS + i, j);
-      };
-      auto full = [&](int f) { return wait(f % kSt, f / kSt); };
-      auto free_stage = [&](int f) { commit(kSt + f % kSt, f / kSt); };
-      if (W.expire) ok = wait(kBarO, 0);  // test only: no product has been issued, so the wait runs out
-      if (ok && nk > 0 && (ok = full(0))) {
-        tc::tc_fence_after();
-        if (nk0 > 0) issue_s(0, 0);
-        if (nk1 > 0) issue_s(1, 0);
-        free_stage(0);
-      }
-      for (int j = 0; j < nk && ok; ++j) {
-        const int fv = 2 * j + 1;
-        ok = full(fv) && (j != fix_tile || wait(kBarFix, 0));
-        const uint32_t v = stage0 + (uint32_t)((fv % kSt) * Geo::kStageBytes);
-        bool next = false;  // K of the next tile has landed
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (j >= (i ? nk1 : nk0)) continue;
-          ok = wait(kBarP + i, j);
-          if (!ok) break;
+            for (int x = 0; x < D / 16; ++x) {
+              const uint32_t off = (uint32_t)((x >> 2) * kBlockBytes);
+              chunk_mma_ss(tmem + 128u * i, tc::sw128_desc(a + off) + 2 * (x & 3), tc::sw128_desc(b + off) + 2 * (x & 3), id_s,
+                           x > 0 ? 1u : 0u);
+            }
+          }
+          commit(kBarS + i, tiles[i] + j);
+        };
+        // The order in which the softmax warps get to them, tile 0's first: S_i of the next keys (with P
+        // apart as soon as this one's columns have been read; in place behind the product that reads
+        // P_i), and P_i V.
+        auto next_s = [&](int i, int j, bool& landed) {
+          if (j >= it.nk[i]) return;
+          if (!landed) ok = full(fills + 2 * j);
+          landed = true;
+          if (Geo::kApart && ok && tiles[i] + j > 0) ok = wait(kBarR + i, tiles[i] + j - 1);
+          if (!ok) return;
           tc::tc_fence_after();
+          issue_s(i, j);
+        };
+        auto done_s = [&](int j) {  // every row tile's S of key tile j has been issued
+          free_stage(fills + 2 * j);
+          if (j + 1 == nk) commit(kQEmpty + q, qs / kQb);
+        };
+        if (nk > 0) {
+          ok = wait(kQFull + q, qs / kQb);
+          bool landed = false;
+          for (int i = 0; i < 2 && ok; ++i) next_s(i, 0, landed);
+          if (ok) done_s(0);
+        }
+        for (int j = 0; j < nk && ok; ++j) {
+          const int fv = fills + 2 * j + 1;
+          const uint32_t v = stage0 + (uint32_t)(fv % kSt * Geo::kStageBytes);
+          bool landed = false;  // K of the next tile
+          for (int i = 0; i < 2 && ok; ++i) {
+            if (Geo::kApart) next_s(i, j + 1, landed);
+            if (!ok || j >= it.nk[i]) continue;
+            if (j == 0 && reads[i] > 0) ok = wait(kBarE + i, reads[i] - 1);  // O_i of the item before has been read
+            ok = ok && full(fv);
 #pragma unroll
-          for (int k = 0; k < kTileKeys / 16; ++k)  // 16 keys: 8 columns of P, 2048 bytes of V
-            tc::tc_mma_ts(tmem + 256u + 128u * i, tmem + 128u * i + 8u * k, mn_desc(v + 2048u * k), id_o,
-                          (j > 0 || k > 0) ? 1u : 0u);
-          commit(kBarO + i, j);
-          if (j + 1 < (i ? nk1 : nk0)) {
-            if (!next) ok = full(2 * j + 2);
-            next = true;
+            for (int half = 0; half < 2 && ok; ++half) {
+              ok = wait(kBarP + 2 * i + half, tiles[i] + j);
+              if (!ok) break;
+              tc::tc_fence_after();
+              if (leader) {
+#pragma unroll
+                for (int x = 4 * half; x < 4 * half + 4; ++x)  // 16 keys: 8 columns of P, 2048 bytes of V
+                  tc::tc_mma_ts(tmem + Geo::kColO + (uint32_t)(D * i), tmem + Geo::kColP + Geo::kStepP * i + 8u * x,
+                                mn_desc(v + 2048u * x), id_o, (j > 0 || x > 0) ? 1u : 0u);
+              }
+            }
             if (!ok) break;
-            tc::tc_fence_after();
-            issue_s(i, j + 1);
+            commit(kBarO + i, tiles[i] + j);
+            if (!Geo::kApart) next_s(i, j + 1, landed);
           }
-        }
-        if (ok) {
+          if (!ok) break;
           free_stage(fv);
-          if (j + 1 < nk) free_stage(2 * j + 2);
+          if (j + 1 < nk) done_s(j + 1);
         }
+        if (!ok) break;
+        fills += 2 * nk;
+        for (int i = 0; i < 2; ++i) {
+          tiles[i] += it.nk[i];
+          reads[i] += it.nk[i] > 0 ? 1 : 0;
+        }
+        qs += nk > 0 ? 1 : 0;
       }
-      if (s_abort && last >= 0) chunk_drain(bar(last), (uint32_t)last_parity, W);
+      // the last commit covers every product before it: none outlives the tensor and shared memory
+      if (last >= 0) chunk_drain(bar(last), (uint32_t)last_parity, W);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
-    // ---- softmax of tile i, a thread per row ----
+    // ---- softmax of row tile i, a thread per row ----
     const int i = warp >> 2;
-    const int nki = i ? nk1 : nk0;
-    const int r = row0 + i * kTileRows + (tid & 127);
-    const int rc = min(r, R - 1);  // rows past the end see what the last one does
-    const int lim = shift + rc / G;
-    const int lim_first = shift + (row0 + i * kTileRows) / G;
     const float c = fmaxf(fabsf(scale) * 1.44269504f, 1e-30f);  // > 0: a masked -inf stays -inf
-    const uint32_t t_s = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128u * i;
-    const uint32_t t_o = t_s - 128u * i + 256u + 128u * i;
-    float m = -INFINITY, l[2] = {0.0f, 0.0f};  // the maximum that O and l are scaled by; the sum's two halves
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const uint32_t t_s = lanes + 128u * i, t_p = lanes + Geo::kColP + Geo::kStepP * i, t_o = lanes + Geo::kColO + (uint32_t)(D * i);
     bool ok = true;
-    for (int j = 0; j < nki; ++j) {
-      ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarS + i), (uint32_t)j & 1u, &s_abort, W));
+    int tiles = 0, all_tiles = 0, k = 0;
+    auto wait = [&](int b, int n) { return __all_sync(0xffffffffu, chunk_wait(bar(b), (uint32_t)n & 1u, &s_abort, W)); };
+    for (;; ++k) {
+      ok = wait(kItem + (k & 1), k / 2);
       if (!ok) break;
-      tc::tc_fence_after();
-      uint32_t u[4][32];  // the row's 128 scores
+      const Item it = s_item[k & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive_n(bar(kItemFree + (k & 1)), 1);
+      if (it.seq < 0) break;
+      const Row row = row_of(it, R, i, tid & 127);
+      const int nk = i ? it.nk[1] : it.nk[0];
+      float m = -INFINITY, l = 0.0f;  // the maximum that O and l are scaled by, and the sum
+      for (int j = 0; j < nk; ++j, ++tiles) {
+        ok = wait(kBarS + i, tiles);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const int rel = row.lim - (it.k_lo + j * kTileKeys);  // keys 0 .. rel of the tile are seen
+        const uint32_t live = s_live[(all_tiles + j) & 15];
+        const bool masked = it.k_lo + j * kTileKeys + kTileKeys - 1 > row.lim_first || live != 0xffu;
+        // two passes over S, half a tile at a time (the loops are not unrolled: with the code of all 128
+        // keys in a row the other warps' instructions no longer stay in the cache)
+        float mt = -INFINITY;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t u[2][32];
+          tc::tmem_ld32(t_s + 64u * half, u[0]);
+          tc::tmem_ld32(t_s + 64u * half + 32u, u[1]);
+          tc::tmem_wait_ld();
+          if (masked) {
+            const int r = rel - 64 * half;
+            const uint32_t lv = live >> (4 * half);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) tc::tmem_ld32(t_s + 32u * x, u[x]);
-      tc::tmem_wait_ld();
-      const int key0 = k_lo + j * kTileKeys;
-      if (key0 + kTileKeys - 1 > lim_first) {
-        const int rel = lim - key0;
+            for (int x = 0; x < 64; ++x) u[x >> 5][x & 31] = x <= r && ((lv >> (x / 16)) & 1u) ? u[x >> 5][x & 31] : kNegInf;
+          }
+          float mx[4];
 #pragma unroll
-        for (int x = 0; x < kTileKeys; ++x) u[x >> 5][x & 31] = x <= rel ? u[x >> 5][x & 31] : kNegInf;
-      }
-      if (any_bad) {  // bit x: the tile's keys 16 x .. 16 x + 15 have a page
-        const int key = key0 + 16 * (lane & 7);
-        const unsigned live = __ballot_sync(0xffffffffu, key < sp.len && page_at(C, table, key >> C.page_log2) >= 0);
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t* v = &u[x >> 1][16 * (x & 1)];
+            mx[x] = max3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
 #pragma unroll
-        for (int x = 0; x < kTileKeys; ++x) u[x >> 5][x & 31] = (live >> (x / 16)) & 1u ? u[x >> 5][x & 31] : kNegInf;
-      }
-      // maximum, as four chains of three-operand maxima
-      float mx[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        mx[x] = max3(__uint_as_float(u[x][0]), __uint_as_float(u[x][1]), __uint_as_float(u[x][2]));
-#pragma unroll
-        for (int e = 3; e < 31; e += 2) mx[x] = max3(mx[x], __uint_as_float(u[x][e]), __uint_as_float(u[x][e + 1]));
-      }
-      float mt = max3(mx[0], mx[1], mx[2]);
-      mt = max3(mt, mx[3], __uint_as_float(u[0][31]));
-      mt = max3(mt, __uint_as_float(u[1][31]), __uint_as_float(u[2][31]));
-      mt = fmaxf(mt, __uint_as_float(u[3][31]));
-      const bool grow = j == 0 ? mt > m : (mt - m) * c > kLazyLog2;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float alpha = grow ? exp2_approx((m - mt) * c) : 1.0f;
-        m = grow ? mt : m;
-        l[0] *= alpha;
-        l[1] *= alpha;
-        if (j > 0) {
-          ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarO + i), (uint32_t)(j - 1) & 1u, &s_abort, W));
+            for (int e = 3; e < 15; e += 2) mx[x] = max3(mx[x], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+            mx[x] = fmaxf(mx[x], __uint_as_float(v[15]));
+          }
+          mt = max3(mt, max3(mx[0], mx[1], mx[2]), mx[3]);
+        }
+        // the product of the tile before: with P apart it may still read P and write O (in place, S was
+        // computed behind it)
+        if (Geo::kApart && tiles > 0) {
+          ok = wait(kBarO + i, tiles - 1);
           if (!ok) break;
           tc::tc_fence_after();
+        }
+        const bool grow = j == 0 ? mt > m : (mt - m) * c > kLazyLog2;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? exp2_approx((m - mt) * c) : 1.0f;
+          m = grow ? mt : m;
+          l *= alpha;
+          if (j > 0) {
+#pragma unroll 1
+            for (int x = 0; x < D / 16; ++x) {
+              uint32_t v[16];
+              tc::tmem_ld16(t_o + 16u * x, v);
+              tc::tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            uint32_t v[16];
-            tc::tmem_ld16(t_o + 16u * x, v);
-            tc::tmem_wait_ld();
+              for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+              tmem_st16<16>(t_o + 16u * x, v);
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+        const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
+        float2 sum0 = make_float2(0.0f, 0.0f), sum1 = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t u[2][32];
+          tc::tmem_ld32(t_s + 64u * half, u[0]);
+          tc::tmem_ld32(t_s + 64u * half + 32u, u[1]);
+          tc::tmem_wait_ld();
+          if (Geo::kApart && half) {  // S may be overwritten
+            tc::tc_fence_before();
+            mbar_arrive_n(bar(kBarR + i), 1);
+          }
+          float2 y[2][16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-            tmem_st16<16>(t_o + 16u * x, v);
+          for (int x = 0; x < 32; ++x) {
+            float2& w = y[x >> 4][x & 15];
+            w = fma2(make_float2(__uint_as_float(u[x >> 4][2 * (x & 15)]), __uint_as_float(u[x >> 4][2 * (x & 15) + 1])), c2, mc2);
+            if (x % 4 == 1) {
+              w = exp2_poly(w);
+            } else {
+              w.x = exp2_approx(w.x);
+              w.y = exp2_approx(w.y);
+            }
+          }
+          if (masked) {  // weights of keys that are not seen are exactly 0
+            const int r = rel - 64 * half;
+            const uint32_t lv = live >> (4 * half);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              float2& w = y[x >> 4][x & 15];
+              const bool lx = (lv >> (x / 8)) & 1u;
+              w.x = 2 * x <= r && lx ? w.x : 0.0f;
+              w.y = 2 * x + 1 <= r && lx ? w.y : 0.0f;
+            }
+          }
+          uint32_t p[2][16];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const float2 w = y[x >> 4][x & 15];
+            if (x & 1) sum1 = add2(sum1, w);
+            else sum0 = add2(sum0, w);
+            p[x >> 4][x & 15] = pack2<T>(w.x, w.y);
+          }
+          tmem_st16<16>(t_p + 32u * half, p[0]);
+          tmem_st16<16>(t_p + 32u * half + 16u, p[1]);
+          tc::tmem_wait_st();
+          tc::tc_fence_before();
+          mbar_arrive_n(bar(kBarP + 2 * i + half), 1);
+        }
+        l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      }
+      if (ok && nk > 0) {
+        ok = wait(kBarO + i, tiles - 1);
+        tc::tc_fence_after();
+      }
+      if (!ok) break;
+      // ---- result: the row's D outputs, or this split's part of them ----
+      const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // no key: zeros
+      const bool whole = it.used == 1, write = row.live && it.z < it.used;
+      float* pp = part + (((int64_t)row.tok * heads + row.h) * splits + it.z) * (D + 8);
+      O* po = out + (int64_t)row.tok * out_ld + (int64_t)row.h * D;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        uint32_t v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0u;
+        if (nk > 0) {
+          tc::tmem_ld32(t_o + 32u * x, v);
+          tc::tmem_wait_ld();
+        }
+        if (write) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float a[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) a[y] = __uint_as_float(v[e + y]) * (whole ? inv : 1.0f);
+            if (whole) store8(po + 32 * x + e, a);
+            else store8(pp + 32 * x + e, a);
           }
         }
       }
-      const float mc = m == -INFINITY ? 0.0f : m * c;
-      const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
-      float2 sum0 = make_float2(0.0f, 0.0f), sum1 = make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint32_t p[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 y = fma2(make_float2(__uint_as_float(u[x][2 * e]), __uint_as_float(u[x][2 * e + 1])), c2, mc2);
-          y.x = exp2_approx(y.x);
-          y.y = exp2_approx(y.y);
-          if (e & 1) sum1 = add2(sum1, y);
-          else sum0 = add2(sum0, y);
-          p[e] = pack2<T>(y.x, y.y);
-        }
-        tmem_st16<16>(t_s + 16u * x, p);
+      if (write && !whole) *reinterpret_cast<float2*>(pp + D) = make_float2(m == -INFINITY ? m : m * c, l);
+      if (nk > 0) {
+        tc::tc_fence_before();
+        mbar_arrive_n(bar(kBarE + i), 1);
       }
-      l[0] += sum0.x + sum1.x;
-      l[1] += sum0.y + sum1.y;
-      tc::tmem_wait_st();
-      tc::tc_fence_before();
-      mbar_arrive_n(bar(kBarP + i), 1);
+      all_tiles += max(it.nk[0], it.nk[1]);
     }
-    if (ok && nki > 0) {
-      ok = __all_sync(0xffffffffu, chunk_wait(bar(kBarO + i), (uint32_t)(nki - 1) & 1u, &s_abort, W));
-      tc::tc_fence_after();
-    }
-    // ---- result: the row's D outputs, or this split's part of them ----
-    const int tok = sp.first + rc / G, h = g * G + rc % G;
-    const float sum = l[0] + l[1], inv = !ok ? NAN : sum > 0.0f ? 1.0f / sum : 0.0f;
-    float* pp = part + (((int64_t)tok * heads + h) * splits + z) * (D + 8);
-    O* po = out + (int64_t)tok * out_ld + (int64_t)h * D;
-#pragma unroll
-    for (int x = 0; x < D / 32; ++x) {
-      uint32_t v[32];
-#pragma unroll
-      for (int e = 0; e < 32; ++e) v[e] = 0u;
-      if (nki > 0 && ok) {
-        tc::tmem_ld32(t_o + 32u * x, v);
-        tc::tmem_wait_ld();
-      }
-      if (r < R) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          float a[8];
-#pragma unroll
-          for (int y = 0; y < 8; ++y) a[y] = __uint_as_float(v[e + y]);
-          if (used > 1) {
-            store8(pp + 32 * x + e, a);
-          } else {
-#pragma unroll
-            for (int y = 0; y < 8; ++y) a[y] *= inv;
-            store8(po + 32 * x + e, a);
-          }
+    if (!ok) {  // a wait ran out: this item's rows and those of all that would have followed are NaN
+      const int total = count_items(C, cu_q, kv_len, rows, R, small_rows);
+      for (int w = blockIdx.x + k * gridDim.x;; w += gridDim.x) {
+        const Item it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, w);
+        if (it.seq < 0) break;
+        const Row row = row_of(it, R, i, tid & 127);
+        if (!row.live || it.z >= it.used) continue;
+        for (int d = 0; d < D; ++d) out[(int64_t)row.tok * out_ld + (int64_t)row.h * D + d] = from_f32<O>(NAN);
+        if (it.used > 1) {
+          float* pp = part + (((int64_t)row.tok * heads + row.h) * splits + it.z) * (D + 8);
+          for (int d = 0; d < D + 8; ++d) pp[d] = NAN;
         }
       }
     }
-    if (r < R && used > 1)
-      *reinterpret_cast<float2*>(pp + D) = ok ? make_float2(m == -INFINITY ? m : m * c, sum) : make_float2(0.0f, NAN);
   }
   tc::tc_fence_before();
   __syncthreads();

@@ -201,7 +201,9 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   P.sp.per[1] = 1 << 30;
   P.sp.splits[1] = 1;
   if (P.chunk) {
-    const int64_t items = std::max<int64_t>(1, ((int64_t)rows * G + kItemRows - 1) / kItemRows) * kv->kv_heads;
+    const RowTiles R = row_tiles(G);
+    const int64_t tiles = ((int64_t)rows + R.tokens - 1) / R.tokens * R.parts;
+    const int64_t items = std::max<int64_t>(1, (tiles + 1) / 2) * kv->kv_heads;
     int64_t best = -1;
     for (int64_t n = 1; n == 1 || (n <= 32 && keys >= 512 * n && items * n <= kChunkItems); ++n) {
       const int64_t p1 = (keys + n * kTileKeys - 1) / (n * kTileKeys) * kTileKeys;
@@ -220,28 +222,40 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   return P;
 }
 
-// TMA map of a pool: (element, head, row, page), boxes of 64 elements x one head x up to 128 rows of a
-// page, 128-byte swizzle.
-static bool pool_map(CUtensorMap* m, const llama_paged_kv_t* kv, void* pool) {
-  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static const Encode encode = [] {
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// A TMA map of 16-bit elements with 128-byte swizzle; what lies outside reads as zeros.
+static bool make_map(CUtensorMap* m, int type, int rank, const void* at, const cuuint64_t* dims, const cuuint64_t* strides,
+                     const cuuint32_t* box) {
+  static const EncodeTiled encode = [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult st;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &st) != cudaSuccess) fn = nullptr;
-    return reinterpret_cast<Encode>(fn);
+    return reinterpret_cast<EncodeTiled>(fn);
   }();
-  if (!encode) return false;
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return encode &&
+         encode(m, type == LLAMA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank,
+                const_cast<void*>(at), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// A pool as (element, head, row, page): boxes of 64 elements x one head x up to 128 rows of a page.
+static bool pool_map(CUtensorMap* m, const llama_paged_kv_t* kv, const void* pool) {
   const cuuint64_t dims[4] = {(cuuint64_t)kv->head_dim, (cuuint64_t)kv->kv_heads, (cuuint64_t)kv->page_size,
                               (cuuint64_t)kv->num_pages};
   const cuuint64_t strides[3] = {(cuuint64_t)kv->head_stride * 2, (cuuint64_t)kv->row_stride * 2,
                                  (cuuint64_t)kv->page_stride * 2};
   const cuuint32_t box[4] = {64, 1, (cuuint32_t)std::min(kv->page_size, kTileKeys), 1};
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  return encode(m, kv->type == LLAMA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool, dims,
-                strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return make_map(m, kv->type, 4, pool, dims, strides, box);
+}
+// The queries as (element, head, token): boxes of 64 elements x a row tile's heads x its tokens.
+static bool query_map(CUtensorMap* m, const llama_paged_kv_t* kv, const void* q, int64_t q_ld, int heads, int rows) {
+  const RowTiles R = row_tiles(heads / kv->kv_heads);
+  const cuuint64_t dims[3] = {(cuuint64_t)kv->head_dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)kv->head_dim * 2, (cuuint64_t)q_ld * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)R.heads, (cuuint32_t)R.tokens};
+  return make_map(m, kv->type, 3, q, dims, strides, box);
 }
 
 // Device word that a wait which ran out in the chunk form sets (its rows become NaN as well).
@@ -262,15 +276,17 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
   const T* qt = static_cast<const T*>(q);
   O* ot = static_cast<O*>(out);
   if (P.chunk) {
-    const int G = heads / C.kv_heads;
-    const int64_t items = ((int64_t)rows * G + kItemRows - 1) / kItemRows + std::min(C.seqs, rows);
-    const int64_t grid = items * C.kv_heads * P.sp.splits[1];
-    if (grid > 0x7fffffff) return "too many rows";
-    CUtensorMap mk, mv;
-    if (!pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v)) return "tensor maps of the pools could not be made";
+    // two row tiles an item, every sequence's last one perhaps half empty
+    const RowTiles R = row_tiles(heads / C.kv_heads);
+    const int64_t tiles = ((int64_t)rows / R.tokens + std::min(C.seqs, rows)) * R.parts;
+    const int64_t items = (tiles / 2 + std::min(C.seqs, rows)) * C.kv_heads * P.sp.splits[1];
+    if (items > 0x3fffffff) return "too many rows";
+    CUtensorMap mq, mk, mv;
+    if (!query_map(&mq, kv, q, q_ld, heads, rows) || !pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v))
+      return "tensor maps could not be made";
     if (!allow_smem(k_paged_chunk<T, O, D>, ChunkGeo<D>::kSmem, dev)) return "shared memory could not be set";
-    launch(chained, k_paged_chunk<T, O, D>, (unsigned)grid, kChunkThreads, ChunkGeo<D>::kSmem, st, mk, mv, C, qt, q_ld, heads,
-           cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], ot, out_ld,
+    launch(chained, k_paged_chunk<T, O, D>, (unsigned)std::min<int64_t>(items, kSms), kChunkThreads, ChunkGeo<D>::kSmem, st,
+           mq, mk, mv, C, heads, cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], ot, out_ld,
            part + P.sp.part1 * (D + 8), waits);
   }
   if (P.decode) {
@@ -290,9 +306,9 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
 
 // No plan for seqs <= rows needs more: a decode tile is split only while there are fewer than
 // kDecodeCtas (sequence, kv head) pairs, into at most kDecodeCtas + that many splits in all; chunks into
-// at most kChunkItems (item, split) pairs of kItemRows rows.
+// at most kChunkItems (item, split) pairs of two row tiles.
 size_t attention_bytes_max(int head_dim) {
-  return ((size_t)kDecodeRows * 2 * kDecodeCtas + (size_t)kItemRows * kChunkItems) * (head_dim + 8) * sizeof(float);
+  return ((size_t)kDecodeRows * 2 * kDecodeCtas + (size_t)2 * kTileRows * kChunkItems) * (head_dim + 8) * sizeof(float);
 }
 
 const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, int64_t q_ld, int heads,

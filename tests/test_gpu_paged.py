@@ -149,6 +149,12 @@ SHAPES = [
     ("f16", 128, 160, 1, 16, [1, 9], [1000, 260]),                               # more heads per kv head than a tile's rows
     ("f16", 64, 32, 8, 64, [300, 300], [4096, 301]),
     ("bf16", 128, 32, 8, 64, [20], [9000]),                                      # few rows, a long cache: split and joined
+    # many items for every SM: odd numbers of row tiles, tiles without keys, splits that end early, tails
+    ("bf16", 128, 28, 4, 16, [33, 1, 19, 200, 0, 37, 18, 36, 55, 90, 1, 130, 17, 300, 64, 5] * 4,
+     [40, 9, 21, 1999, 3, 37, 333, 36, 60, 1500, 1, 130, 18, 311, 64, 7] * 4),
+    ("f16", 64, 12, 2, 32, [33, 7, 100, 200, 1, 37, 64, 21, 43, 90, 11, 130, 17, 300] * 6,
+     [33, 5, 4000, 201, 9, 37, 64, 400, 44, 3, 1100, 130, 18, 311] * 6),
+    ("f16", 128, 200, 1, 16, [1, 2, 3] * 40, [200, 17, 130] * 40),
 ]
 
 
