@@ -445,100 +445,102 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // ---- products ----
       constexpr uint32_t id_o = chunk_idesc<T>(D, 1);
       const uint32_t id_s = chunk_idesc<T>(kTileKeys, 0) | (scale < 0.0f ? 1u << 13 : 0u);  // A = -Q: |scale| remains
+      // What the products' operands are made of has to be the warp's in the compiler's eyes as well (a
+      // reduction's result is): else every operand goes through a register of one lane.
+      const uint32_t t0 = __reduce_max_sync(0xffffffffu, tmem);
       const bool leader = tc::elect_one();
       bool ok = true;
-      int fills = 0, qs = 0, last = -1, last_parity = 0;
+      int st = 0, ph = 0;  // stage and phase of the next fill (K and V of a tile are two)
+      int q = 0, qp = 0;   // Q buffer and phase of the next item
       int tiles[2] = {0, 0}, reads[2] = {0, 0};  // per row tile: key tiles so far, items that had some
+      int last = -1, last_parity = 0;
       auto wait = [&](int b, int n) { return __all_sync(0xffffffffu, chunk_wait(bar(b), (uint32_t)n & 1u, &s_abort, W)); };
-      auto commit = [&](int b, int n) {  // n: how often this barrier was committed before
+      auto commit = [&](int b, int n) {  // n: the phase that this completes
         if (leader) tc::tc_commit(bar(b));
         last = b;
         last_parity = n & 1;
       };
-      auto full = [&](int f) { return wait(kFull + f % kSt, f / kSt); };
-      auto free_stage = [&](int f) { commit(kEmpty + f % kSt, f / kSt); };
       if (W.expire) ok = wait(kNever, 0);  // test only
       for (int k = 0; ok; ++k) {
         ok = wait(kItem + (k & 1), k / 2);
         if (!ok) break;
-        const Item it = s_item[k & 1];
-        __syncwarp();
+        const bool more = __reduce_max_sync(0xffffffffu, s_item[k & 1].seq) >= 0;
+        const int nk0 = __reduce_max_sync(0xffffffffu, s_item[k & 1].nk[0]), nk1 = __reduce_max_sync(0xffffffffu, s_item[k & 1].nk[1]);
         if (lane == 0) mbar_arrive_n(bar(kItemFree + (k & 1)), 1);
-        if (it.seq < 0) break;
-        const int nk = max(it.nk[0], it.nk[1]);
-        const int q = qs % kQb;
-        // S_i of key tile j; behind it this row tile's count moves on
-        auto issue_s = [&](int i, int j) {
-          const uint32_t a = base + (uint32_t)((2 * q + i) * Geo::kStageBytes);
-          const uint32_t b = stage0 + (uint32_t)((fills + 2 * j) % kSt * Geo::kStageBytes);
+        if (!more) break;
+        const int nk = max(nk0, nk1);
+        if (nk == 0) continue;
+        // S_i from the K in stage s
+        auto issue_s = [&](int i, int j, int s) {
+          const uint32_t a = base + (uint32_t)((2 * q + i) * Geo::kStageBytes), b = stage0 + (uint32_t)(s * Geo::kStageBytes);
+          tc::tc_fence_after();
           if (leader) {
 #pragma unroll
             for (int x = 0; x < D / 16; ++x) {
               const uint32_t off = (uint32_t)((x >> 2) * kBlockBytes);
-              chunk_mma_ss(tmem + 128u * i, tc::sw128_desc(a + off) + 2 * (x & 3), tc::sw128_desc(b + off) + 2 * (x & 3), id_s,
+              chunk_mma_ss(t0 + 128u * i, tc::sw128_desc(a + off) + 2 * (x & 3), tc::sw128_desc(b + off) + 2 * (x & 3), id_s,
                            x > 0 ? 1u : 0u);
             }
           }
           commit(kBarS + i, tiles[i] + j);
         };
-        // The order in which the softmax warps get to them, tile 0's first: S_i of the next keys (with P
-        // apart as soon as this one's columns have been read; in place behind the product that reads
-        // P_i), and P_i V.
-        auto next_s = [&](int i, int j, bool& landed) {
-          if (j >= it.nk[i]) return;
-          if (!landed) ok = full(fills + 2 * j);
-          landed = true;
-          if (Geo::kApart && ok && tiles[i] + j > 0) ok = wait(kBarR + i, tiles[i] + j - 1);
-          if (!ok) return;
-          tc::tc_fence_after();
-          issue_s(i, j);
-        };
-        auto done_s = [&](int j) {  // every row tile's S of key tile j has been issued
-          free_stage(fills + 2 * j);
-          if (j + 1 == nk) commit(kQEmpty + q, qs / kQb);
-        };
-        if (nk > 0) {
-          ok = wait(kQFull + q, qs / kQb);
-          bool landed = false;
-          for (int i = 0; i < 2 && ok; ++i) next_s(i, 0, landed);
-          if (ok) done_s(0);
-        }
+        ok = wait(kQFull + q, qp) && wait(kFull + st, ph);
+        if (!ok) break;
+        if (Geo::kApart && nk0 > 0 && tiles[0] > 0) ok = wait(kBarR + 0, tiles[0] - 1);
+        if (ok && nk0 > 0) issue_s(0, 0, st);
+        if (ok && Geo::kApart && nk1 > 0 && tiles[1] > 0) ok = wait(kBarR + 1, tiles[1] - 1);
+        if (ok && nk1 > 0) issue_s(1, 0, st);
+        if (!ok) break;
+        commit(kEmpty + st, ph);
+        if (nk == 1) commit(kQEmpty + q, qp);
+        if (++st == kSt) st = 0, ++ph;
         for (int j = 0; j < nk && ok; ++j) {
-          const int fv = fills + 2 * j + 1;
-          const uint32_t v = stage0 + (uint32_t)(fv % kSt * Geo::kStageBytes);
-          bool landed = false;  // K of the next tile
-          for (int i = 0; i < 2 && ok; ++i) {
-            if (Geo::kApart) next_s(i, j + 1, landed);
-            if (!ok || j >= it.nk[i]) continue;
-            if (j == 0 && reads[i] > 0) ok = wait(kBarE + i, reads[i] - 1);  // O_i of the item before has been read
-            ok = ok && full(fv);
+          const int sv = st, pv = ph;
+          if (++st == kSt) st = 0, ++ph;
+          const int sk = st, pk = ph;  // K of the next tile
+          const bool next = j + 1 < nk;
+          if (next && ++st == kSt) st = 0, ++ph;
+          const uint32_t v = stage0 + (uint32_t)(sv * Geo::kStageBytes);
+          ok = wait(kFull + sv, pv) && (!next || wait(kFull + sk, pk));
+          // the order in which the softmax warps get to them: P_i V and S_i of the next keys (with P apart
+          // as soon as this one's columns have been read; in place behind the product that reads P_i)
 #pragma unroll
-            for (int half = 0; half < 2 && ok; ++half) {
-              ok = wait(kBarP + 2 * i + half, tiles[i] + j);
+          for (int i = 0; i < 2; ++i) {
+            const int nki = i ? nk1 : nk0;
+            if (!ok || j >= nki) continue;
+            if (Geo::kApart && j + 1 < nki) {
+              ok = wait(kBarR + i, tiles[i] + j);
+              if (!ok) continue;
+              issue_s(i, j + 1, sk);
+            }
+            if (j == 0 && reads[i] > 0) ok = wait(kBarE + i, reads[i] - 1);  // O_i of the item before has been read
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              ok = ok && wait(kBarP + 2 * i + half, tiles[i] + j);
               if (!ok) break;
               tc::tc_fence_after();
               if (leader) {
 #pragma unroll
                 for (int x = 4 * half; x < 4 * half + 4; ++x)  // 16 keys: 8 columns of P, 2048 bytes of V
-                  tc::tc_mma_ts(tmem + Geo::kColO + (uint32_t)(D * i), tmem + Geo::kColP + Geo::kStepP * i + 8u * x,
+                  tc::tc_mma_ts(t0 + Geo::kColO + (uint32_t)(D * i), t0 + Geo::kColP + Geo::kStepP * i + 8u * x,
                                 mn_desc(v + 2048u * x), id_o, (j > 0 || x > 0) ? 1u : 0u);
               }
             }
-            if (!ok) break;
+            if (!ok) continue;
             commit(kBarO + i, tiles[i] + j);
-            if (!Geo::kApart) next_s(i, j + 1, landed);
+            if (!Geo::kApart && j + 1 < nki) issue_s(i, j + 1, sk);
           }
           if (!ok) break;
-          free_stage(fv);
-          if (j + 1 < nk) done_s(j + 1);
+          commit(kEmpty + sv, pv);
+          if (next) commit(kEmpty + sk, pk);
+          if (j + 2 == nk) commit(kQEmpty + q, qp);
         }
         if (!ok) break;
-        fills += 2 * nk;
-        for (int i = 0; i < 2; ++i) {
-          tiles[i] += it.nk[i];
-          reads[i] += it.nk[i] > 0 ? 1 : 0;
-        }
-        qs += nk > 0 ? 1 : 0;
+        tiles[0] += nk0;
+        tiles[1] += nk1;
+        reads[0] += nk0 > 0 ? 1 : 0;
+        reads[1] += nk1 > 0 ? 1 : 0;
+        if (++q == kQb) q = 0, ++qp;
       }
       // the last commit covers every product before it: none outlives the tensor and shared memory
       if (last >= 0) chunk_drain(bar(last), (uint32_t)last_parity, W);
