@@ -196,18 +196,21 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   per = std::max<int64_t>(64, (per + 63) / 64 * 64);
   P.sp.per[0] = (int)per;
   P.sp.splits[0] = P.decode ? (int)((keys + per - 1) / per) : 1;
-  // chunk: one CTA per SM; as many splits as make the estimated waves x (a split's keys + the fixed
-  // cost of an item, about that of 256 keys) smallest, at least 512 keys each
+  // chunk: one CTA per SM; as many splits as make the estimate smallest: the busiest SM's key tiles,
+  // three more for each of its items, and the parts' way through memory, of which about 8 MB pass in the
+  // 1.9 us of a key tile.  512 tokens over 32768 keys (8 x 8 items): 2 splits 251 us, 9 (which would
+  // fill the SMs better) 290 us.
   P.sp.per[1] = 1 << 30;
   P.sp.splits[1] = 1;
   if (P.chunk) {
     const RowTiles R = row_tiles(G);
     const int64_t tiles = ((int64_t)rows + R.tokens - 1) / R.tokens * R.parts;
     const int64_t items = std::max<int64_t>(1, (tiles + 1) / 2) * kv->kv_heads;
-    int64_t best = -1;
+    const double part_tiles = (double)rows * heads * (kv->head_dim + 8) * 8 / 8e6;
+    double best = -1;
     for (int64_t n = 1; n == 1 || (n <= 32 && keys >= 512 * n && items * n <= kChunkItems); ++n) {
       const int64_t p1 = (keys + n * kTileKeys - 1) / (n * kTileKeys) * kTileKeys;
-      const int64_t cost = (items * n + kSms - 1) / kSms * (p1 + 256);
+      const double cost = (double)((items * n + kSms - 1) / kSms) * (p1 / kTileKeys + 3) + (n > 1 ? 2 + n * part_tiles : 0);
       if (best < 0 || cost < best) {
         best = cost;
         P.sp.per[1] = n == 1 ? 1 << 30 : (int)p1;
