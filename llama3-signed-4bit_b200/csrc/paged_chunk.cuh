@@ -7,7 +7,8 @@
 // (token-major); a row tile is the 128 / G whole tokens that fit the 128 rows of an MMA (G > 128: 128
 // of a token's heads), and a work item two row tiles of one sequence and kv head, so that every key is
 // read once for up to 256 rows.  One CTA per SM takes items in turn, the longest of each sequence
-// first, and walks an item's keys in tiles of 128:
+// first (a CTA that is done takes over the next one of the grid that has not started), and walks an
+// item's keys in tiles of 128:
 //
 //   * warp 9 finds the items and runs ahead of the others: it publishes an item's description, brings Q
 //     (one box of heads x tokens per column block) and then the K and V rows tile by tile into a ring
@@ -33,8 +34,8 @@
 // that.
 //
 // All mbarrier waits are bounded; on timeout the error word is set, every role stops, the copies and
-// products in flight are waited for (again bounded) and the rows of the CTA's remaining items become
-// NaN.
+// products in flight are waited for (again bounded) and the rows of the items that the CTA had taken on
+// become NaN.
 #pragma once
 
 #include <cuda.h>
@@ -172,6 +173,27 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
+// Takes over a CTA of this grid that has not started (16 bytes to shared memory, on a barrier): the SM
+// that is done first gets the next item, without a counter in memory.
+__device__ __forceinline__ void steal_cta(uint32_t to, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(to),
+               "r"(bar)
+               : "memory");
+}
+// Its block index, or -1 when every CTA has started.
+__device__ __forceinline__ int stolen_cta(uint32_t from) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(from)
+      : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read before the next one is written
+  return got ? (int)x : -1;
+}
+
 // How rows are cut into tiles: `tokens` tokens of `heads` heads a tile, `parts` tiles across a token's
 // heads (more than one only for G > 128).
 struct RowTiles {
@@ -202,6 +224,7 @@ __device__ __forceinline__ Item find_item(const Cache& C, const int32_t* cu_q, c
   const int lane = threadIdx.x & 31;
   Item it;
   it.seq = -1;
+  if (w < 0) return it;
   it.g = w % C.kv_heads;
   it.z = (w / C.kv_heads) % splits;
   const int want = total - 1 - w / C.kv_heads / splits;
@@ -276,7 +299,7 @@ __device__ __forceinline__ Row row_of(const Item& it, const RowTiles& T, int i, 
   return x;
 }
 
-// Grid: one CTA per SM (fewer when there are fewer items).  per: keys of a split, a multiple of 128.
+// Grid: at least one CTA for every item x split x kv head (find_item's order).  per: keys of a split, a multiple of 128.
 // Sequences of at most small_rows rows per kv head are the decode form's.
 template <typename T, typename O, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
@@ -291,9 +314,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // ready, S read, P halves, O done, O read; the loader's own for a V tail; one that nothing completes
   constexpr int kFull = 0, kEmpty = kSt, kItem = 2 * kSt, kItemFree = kItem + 2, kQFull = kItemFree + 2, kQEmpty = kQFull + kQb;
   constexpr int kBarS = kQEmpty + kQb, kBarR = kBarS + 2, kBarP = kBarR + 2, kBarO = kBarP + 4, kBarE = kBarO + 2;
-  constexpr int kBarFix = kBarE + 2, kNever = kBarFix + 1, kBars = kNever + 1;
+  constexpr int kBarFix = kBarE + 2, kNever = kBarFix + 1, kSteal = kNever + 1, kBars = kSteal + 1;
   __shared__ __align__(8) unsigned long long s_bar[kBars];
   __shared__ Item s_item[2];
+  __shared__ __align__(16) uint32_t s_steal[4];
+  __shared__ volatile int s_claimed[4], s_claims;  // the launch's items that this CTA has taken on: the last four, how many
   __shared__ uint32_t s_tmem;
   __shared__ volatile uint32_t s_abort;
   __shared__ volatile uint32_t s_live[16];  // per key tile: bit x, its keys 16 x .. 16 x + 15 have a page
@@ -301,6 +326,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   auto bar = [&](int i) { return smem_u32(&s_bar[i]); };
   if (tid == 0) {
     s_abort = 0u;
+    s_claims = 0;
     for (int i = 0; i < kBars; ++i) {
       const bool half = (i >= kBarR && i < kBarO) || (i >= kBarE && i < kBarFix);       // a row tile's threads
       mbar_init(bar(i), half ? kTileRows : i == kItemFree || i == kItemFree + 1 ? 10 : 1);  // the item's readers
@@ -321,6 +347,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t base = (smem_u32(chunk_smem) + 1023u) & ~1023u;  // Q buffers of two row tiles, then the stages
   const uint32_t stage0 = base + (uint32_t)(2 * kQb * Geo::kStageBytes);
   const int page_mask = (1 << C.page_log2) - 1;
+  int item = 1 << 30;  // the item that a wait which ran out ended
   if (warp >= 8) {
     if (warp >= 9) {
       // ---- loaders: K (and the items and Q), V ----
@@ -332,11 +359,37 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       bool ok = true;
       int fills = 0, tiles = 0, fixes = 0, qs = 0, last = -1;  // fills: K and V of a tile are two
       auto wait = [&](int b, int n) { return __all_sync(0xffffffffu, chunk_wait(bar(b), (uint32_t)n & 1u, &s_abort, W)); };
-      for (int w = blockIdx.x, k = 0; ok; w += gridDim.x, ++k) {
+      int w = blockIdx.x, steals = 0;
+      auto steal = [&] {
+        if (leader) {
+          mbar_expect_tx(bar(kSteal), 16);
+          steal_cta(smem_u32(s_steal), bar(kSteal));
+        }
+        ++steals;
+      };
+      auto stolen = [&] {  // the next item; -1: no more, or a wait ran out
+        ok = wait(kSteal, steals - 1);
+        w = ok ? stolen_cta(smem_u32(s_steal)) : -1;
+        __syncwarp();
+      };
+      for (int k = 0; ok; ++k) {
         Item it;
         if (kv == 0) {
-          it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, w);
-          if (k >= 2) ok = wait(kItemFree + (k & 1), k / 2 - 1);
+          do {  // past the last item the launch has CTAs without work
+            it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, w);
+            if (it.seq < 0 && w >= 0) {
+              steal();
+              stolen();
+            }
+          } while (ok && it.seq < 0 && w >= 0);
+          if (it.seq >= 0) {
+            if (leader) {
+              s_claimed[k & 3] = w;
+              s_claims = k + 1;
+            }
+            steal();  // the answer is there when this item has been loaded
+          }
+          if (ok && k >= 2) ok = wait(kItemFree + (k & 1), k / 2 - 1);
           if (!ok) break;
           if (leader) {
             s_item[k & 1] = it;
@@ -351,7 +404,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         if (it.seq < 0) break;
         const int nk = max(it.nk[0], it.nk[1]);
-        if (nk == 0) continue;
+        if (nk == 0) {
+          if (kv == 0) stolen();
+          continue;
+        }
         if (kv == 0) {
           if (qs >= kQb) ok = wait(kQEmpty + qs % kQb, qs / kQb - 1);
           if (!ok) break;
@@ -435,11 +491,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           entry = next;
         }
         fills += 2 * nk;
+        if (kv == 0 && ok) stolen();
       }
       if (s_abort) {  // the copies in flight land before the shared memory goes
         for (int f = last; f >= 0 && f > last - kSt; f -= 2) chunk_drain(bar(kFull + f % kSt), (uint32_t)(f / kSt) & 1u, W);
         for (int f = max(0, qs - kQb); f < qs; ++f) chunk_drain(bar(kQFull + f % kQb), (uint32_t)(f / kQb) & 1u, W);
         if (fixes > 0) chunk_drain(bar(kBarFix), (uint32_t)(fixes - 1) & 1u, W);
+        if (steals > 0) {  // an item that was taken on but not begun is among those that become NaN
+          chunk_drain(bar(kSteal), (uint32_t)(steals - 1) & 1u, W);
+          const int next = w >= 0 || !ok ? stolen_cta(smem_u32(s_steal)) : -1;
+          const int n = s_claims;
+          __syncwarp();
+          if (leader && next >= 0 && (n == 0 || s_claimed[(n - 1) & 3] != next)) {
+            s_claimed[n & 3] = next;
+            s_claims = n + 1;
+          }
+        }
       }
     } else if (warp == 8) {
       // ---- products ----
@@ -711,23 +778,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       all_tiles += max(it.nk[0], it.nk[1]);
     }
-    if (!ok) {  // a wait ran out: this item's rows and those of all that would have followed are NaN
-      const int total = count_items(C, cu_q, kv_len, rows, R, small_rows);
-      for (int w = blockIdx.x + k * gridDim.x;; w += gridDim.x) {
-        const Item it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, w);
-        if (it.seq < 0) break;
-        const Row row = row_of(it, R, i, tid & 127);
-        if (!row.live || it.z >= it.used) continue;
-        for (int d = 0; d < D; ++d) out[(int64_t)row.tok * out_ld + (int64_t)row.h * D + d] = from_f32<O>(NAN);
-        if (it.used > 1) {
-          float* pp = part + (((int64_t)row.tok * heads + row.h) * splits + it.z) * (D + 8);
-          for (int d = 0; d < D + 8; ++d) pp[d] = NAN;
-        }
-      }
-    }
+    item = ok ? 1 << 30 : k;
   }
   tc::tc_fence_before();
   __syncthreads();
+  // a wait ran out: the rows of the item it ended, and of those that this CTA had taken on behind it, are NaN
+  if (s_abort && warp < 8) {
+    const int i = warp >> 2, total = count_items(C, cu_q, kv_len, rows, R, small_rows);
+    for (int k = item; k < s_claims; ++k) {
+      const Item it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, s_claimed[k & 3]);
+      if (it.seq < 0) continue;
+      const Row row = row_of(it, R, i, tid & 127);
+      if (!row.live || it.z >= it.used) continue;
+      for (int d = 0; d < D; ++d) out[(int64_t)row.tok * out_ld + (int64_t)row.h * D + d] = from_f32<O>(NAN);
+      if (it.used > 1) {
+        float* pp = part + (((int64_t)row.tok * heads + row.h) * splits + it.z) * (D + 8);
+        for (int d = 0; d < D + 8; ++d) pp[d] = NAN;
+      }
+    }
+  }
   if (warp == 8) {
     __syncwarp();
     tc::tc_fence_after();

@@ -288,7 +288,7 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
     if (!query_map(&mq, kv, q, q_ld, heads, rows) || !pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v))
       return "tensor maps could not be made";
     if (!allow_smem(k_paged_chunk<T, O, D>, ChunkGeo<D>::kSmem, dev)) return "shared memory could not be set";
-    launch(chained, k_paged_chunk<T, O, D>, (unsigned)std::min<int64_t>(items, kSms), kChunkThreads, ChunkGeo<D>::kSmem, st,
+    launch(chained, k_paged_chunk<T, O, D>, (unsigned)items, kChunkThreads, ChunkGeo<D>::kSmem, st,
            mq, mk, mv, C, heads, cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], ot, out_ld,
            part + P.sp.part1 * (D + 8), waits);
   }
