@@ -1463,7 +1463,7 @@ static bool init_device(Engine* E, const uint8_t* base, const ParsedFile& P) {
       if (E->err.empty()) E->err = "a paged engine needs the tensor-core batched path";
       return false;
     }
-    LE_CK(cudaMalloc(&E->paged_ws, paged::attention_bytes_max(LE_HEAD_DIM)));
+    LE_CK(cudaMalloc(&E->paged_ws, paged::attention_bytes_max(LE_HEAD_DIM, (int)E->kv_heads, E->tc_T, E->page_width * E->page_size)));
   }
   return true;
 }

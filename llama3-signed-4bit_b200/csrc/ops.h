@@ -68,7 +68,8 @@ const char* append_rows(const llama_paged_kv_t* kv, const void* qkv, int type, i
                         int64_t plane_stride, int rows, int heads, const int32_t* pos, const int32_t* seq,
                         const float* rope_cos, const float* rope_sin, int n_pos, void* q_out, int q_type, int64_t q_ld,
                         cudaStream_t st, bool chained);
-size_t attention_bytes_max(int head_dim);  // workspace that covers every call with seqs <= rows
+// Workspace that covers every call of at most seqs <= rows sequences and max_kv keys.
+size_t attention_bytes_max(int head_dim, int kv_heads, int seqs, int max_kv);
 const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, int64_t q_ld, int heads,
                            const int32_t* cu_q, const int32_t* kv_len, int rows, int max_q, int max_kv, float scale,
                            void* out, int out_type, int64_t out_ld, void* workspace, const Waits& waits, cudaStream_t st,

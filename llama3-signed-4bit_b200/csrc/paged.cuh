@@ -140,46 +140,78 @@ struct SplitPlan {
   int64_t part1;
 };
 
-// out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the splits of a (row, head), M = max m_z.
-// D / 8 threads per (row, head); rows whose sequence has one split were written already.
+// out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the splits of a (row, head), M = max m_z;
+// rows whose sequence has one split were written already.  D / 8 << groups_log2 threads per (row,
+// head), 8 outputs each: a group of D / 8 takes every groups-th split with a running (M, L, o), and
+// the groups join through shared memory.  A thread's loads follow one another's addresses only, so
+// kCombineRun splits are in flight at a time.
+constexpr int kCombineThreads = 128, kCombineRun = 4;
 template <typename O, int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kCombineThreads)
     k_paged_combine(Cache C, int heads, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ kv_len, int rows,
-                    SplitPlan P, const float* __restrict__ part, O* __restrict__ out, int64_t out_ld) {
+                    SplitPlan P, int groups_log2, const float* __restrict__ part, O* __restrict__ out, int64_t out_ld) {
   grid_dep_wait();  // the parts come from the kernel before
   constexpr int kRuns = D / 8;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t rh = i / kRuns;
-  if (rh >= (int64_t)rows * heads) return;
-  const int d = (int)(i % kRuns) * 8, t = (int)(rh / heads), h = (int)(rh % heads);
-  int lo = 0, hi = C.seqs;  // sequence of row t: the first whose end lies behind it
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cu_q[mid + 1] <= t) lo = mid + 1;
-    else hi = mid;
+  __shared__ __align__(16) float s_a[kCombineThreads][8];
+  __shared__ float2 s_ml[kCombineThreads];
+  const int groups = 1 << groups_log2, mine = threadIdx.x % kRuns, grp = threadIdx.x / kRuns % groups;
+  const int64_t rh = ((int64_t)blockIdx.x * kCombineThreads + threadIdx.x) / (kRuns * groups);
+  const int d = mine * 8, t = (int)(rh / heads), h = (int)(rh % heads);
+  int used = 0;  // splits to join: none where the row is nobody's, or has been written
+  const float* p = part;
+  if (t < rows) {
+    int lo = 0, hi = C.seqs;  // sequence of row t: the first whose end lies behind it
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (cu_q[mid + 1] <= t) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo < C.seqs) {
+      const Span sp = span_of(C, cu_q, kv_len, lo, rows);
+      const int G = heads / C.kv_heads, kind = sp.n * G <= P.small_rows ? 0 : 1;
+      const int S = P.splits[kind];
+      used = t < sp.first ? 0 : splits_of(sp.len, P.per[kind], S);
+      if (used > 1)
+        p += (kind ? P.part1 + rh * S : (((int64_t)lo * C.kv_heads + h / G) * kDecodeRows + (t - sp.first) * G + h % G) * S) *
+             (D + 8);
+    }
   }
-  if (lo >= C.seqs) return;
-  const Span sp = span_of(C, cu_q, kv_len, lo, rows);
-  if (t < sp.first) return;
-  const int G = heads / C.kv_heads, kind = sp.n * G <= P.small_rows ? 0 : 1;
-  const int S = P.splits[kind], used = splits_of(sp.len, P.per[kind], S);
-  if (used <= 1) return;
-  const int64_t index = kind ? P.part1 + rh * S
-                             : (((int64_t)lo * C.kv_heads + h / G) * kDecodeRows + (t - sp.first) * G + h % G) * S;
-  const float* p = part + index * (D + 8);
-  float M = -INFINITY;
-  for (int z = 0; z < used; ++z) M = fmaxf(M, p[(int64_t)z * (D + 8) + D]);
-  float L = 0.0f, a[8] = {};
-  for (int z = 0; z < used; ++z) {
-    const float* pz = p + (int64_t)z * (D + 8);
-    const float2 ml = *reinterpret_cast<const float2*>(pz + D);
-    const float f = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - M);
-    float x[8];
-    load8(pz + d, x);
-    L = fmaf(ml.y, f, L);
+  float M = -INFINITY, L = 0.0f, a[8] = {};
+  auto join = [&](float2 ml, const float (&x)[8]) {
+    const float m = fmaxf(M, ml.x);
+    const float f = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - m), g = M == -INFINITY ? 0.0f : exp2_approx(M - m);
+    M = m;
+    L = fmaf(ml.y, f, L * g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = fmaf(x[e], f, a[e]);
+    for (int e = 0; e < 8; ++e) a[e] = fmaf(x[e], f, a[e] * g);
+  };
+  if (used > 1) {
+    for (int z0 = grp; z0 < used; z0 += kCombineRun * groups) {
+      float2 ml[kCombineRun];
+      float x[kCombineRun][8];
+#pragma unroll
+      for (int i = 0; i < kCombineRun; ++i) {
+        const float* pz = p + (int64_t)min(z0 + i * groups, used - 1) * (D + 8);
+        ml[i] = *reinterpret_cast<const float2*>(pz + D);
+        load8(pz + d, x[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kCombineRun; ++i)
+        if (z0 + i * groups < used) join(ml[i], x[i]);
+    }
   }
+  if (groups > 1) {  // the block's own (row, head)s: all threads come here
+    store8(s_a[threadIdx.x], a);
+    s_ml[threadIdx.x] = make_float2(M, L);
+    __syncthreads();
+    if (grp) return;
+    for (int y = 1; y < groups; ++y) {
+      float x[8];
+      load8(s_a[threadIdx.x + y * kRuns], x);
+      join(s_ml[threadIdx.x + y * kRuns], x);
+    }
+  }
+  if (used <= 1) return;
   const float inv = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) a[e] *= inv;

@@ -17,12 +17,15 @@
 //     XOR-swizzled by row so that ldmatrix is free of conflicts): no barrier between the warps until
 //     they merge their (m, l, o) at the end.  Rows past the length are zero-filled: what stale
 //     memory holds there meets weights of 0 and must not be NaN.
-//   * With several splits a CTA writes its unnormalised (m, l, o) in fp32, and k_paged_combine
-//     joins the splits of a row; a sequence that fits one split is written at once.
+//   * Up to eight splits of a sequence and kv head are one thread-block cluster, whose CTAs join their
+//     unnormalised (m, l, o) through distributed shared memory.  More of them (few sequences with many
+//     keys) write them in fp32 and k_paged_combine joins them.  A sequence that fits one split is
+//     written at once.
 // The weights are rounded to the cache's type for the product with v (the type its v has), the sum
 // l takes them unrounded in fp32.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -35,6 +38,7 @@ namespace paged {
 
 constexpr int kSlice = 16;        // keys a warp takes at a time
 constexpr int kDecodeWarps = 4;
+constexpr int kJoinSplits = 8;    // splits that a cluster joins
 template <int D> struct DecodeGeo {
   static constexpr int kStages = D == 64 ? 4 : 3;              // slices in flight per warp
   static constexpr int kSliceBytes = kSlice * D * 2;           // K (or V) of a slice
@@ -66,9 +70,10 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, 
 }
 
 // Grid: seqs x splits x kv_heads, kv heads fastest (their CTAs read neighbouring bytes of the same
-// rows).  per: keys of a split, a multiple of 64; the last split takes all keys behind it.  beside:
-// launched while the chunk form of the same call runs, whose inputs are complete.
-template <typename T, typename O, int D>
+// rows); kJoin: seqs x kv_heads x splits, the splits of a pair a cluster.  per: keys of a split, a
+// multiple of 64; the last split takes all keys behind it.  beside: launched while the chunk form of
+// the same call runs, whose inputs are complete.
+template <typename T, typename O, int D, bool kJoin>
 __global__ void __launch_bounds__(32 * kDecodeWarps)
     k_paged_decode(Cache C, const T* __restrict__ q, int64_t q_ld, int heads, const int32_t* __restrict__ cu_q,
                    const int32_t* __restrict__ kv_len, int rows, float scale_log2, int per, int splits, int beside,
@@ -80,13 +85,18 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
   grid_dep_launch();
   if (!beside) grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = blockIdx.x % C.kv_heads;
-  const int z = (blockIdx.x / C.kv_heads) % splits;
+  const int z = kJoin ? blockIdx.x % splits : (blockIdx.x / C.kv_heads) % splits;
+  const int g = (kJoin ? blockIdx.x / splits : blockIdx.x) % C.kv_heads;
   const int s = blockIdx.x / C.kv_heads / splits;
   const Span sp = span_of(C, cu_q, kv_len, s, rows);
   const int G = heads / C.kv_heads, R = sp.n * G;
   const int used = splits_of(sp.len, per, splits);
+  namespace cg = cooperative_groups;
   if (sp.n <= 0 || R > kDecodeRows || z >= used) {  // nothing to do, or the chunk form's
+    if (kJoin && sp.n > 0 && R <= kDecodeRows && used > 1) {  // the others of the cluster join
+      cg::this_cluster().sync();
+      cg::this_cluster().sync();
+    }
     grid_dep_wait();
     return;
   }
@@ -255,28 +265,68 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
   }
   __syncthreads();
   constexpr int kPer = 8;  // elements a thread merges at a time
-  for (int i = threadIdx.x; i < R * (D / kPer); i += blockDim.x) {
-    const int r = i / (D / kPer), d = (i % (D / kPer)) * kPer;
-    float M = s_m[0][r];
+  constexpr int kItems = kDecodeRows * D / kPer / (32 * kDecodeWarps);  // of them at most
+  const int items = R * (D / kPer);
+  auto finish = [&](int i, float L, float (&a)[kPer]) {
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;  // no key: zeros
 #pragma unroll
-    for (int w = 1; w < kDecodeWarps; ++w) M = fmaxf(M, s_m[w][r]);
-    float L = 0.0f, a[kPer] = {};
+    for (int e = 0; e < kPer; ++e) a[e] *= inv;
+    const int r = i / (D / kPer);
+    store8(out + (int64_t)(sp.first + r / G) * out_ld + (int64_t)(g * G + r % G) * D + i % (D / kPer) * kPer, a);
+  };
+  float M[kItems], L[kItems], a[kItems][kPer];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int i = threadIdx.x + k * 32 * kDecodeWarps, r = i / (D / kPer), d = i % (D / kPer) * kPer;
+    if (i >= items) break;
+    M[k] = s_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kDecodeWarps; ++w) M[k] = fmaxf(M[k], s_m[w][r]);
+    L[k] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) a[k][e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < kDecodeWarps; ++w) {
-      const float f = s_m[w][r] == -INFINITY ? 0.0f : exp2_approx(s_m[w][r] - M);
-      L = fmaf(s_l[w][r], f, L);
+      const float f = s_m[w][r] == -INFINITY ? 0.0f : exp2_approx(s_m[w][r] - M[k]);
+      L[k] = fmaf(s_l[w][r], f, L[k]);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) a[e] = fmaf(so[(w * kDecodeRows + r) * D + d + e], f, a[e]);
+      for (int e = 0; e < kPer; ++e) a[k][e] = fmaf(so[(w * kDecodeRows + r) * D + d + e], f, a[k][e]);
     }
-    const int t = sp.first + r / G, h = g * G + r % G;
-    if (used > 1) {
-      write_part<D>(part, (((int64_t)s * C.kv_heads + g) * kDecodeRows + r) * splits + z, d, M, L, a);
-    } else {
-      const float inv = L > 0.0f ? 1.0f / L : 0.0f;  // no key: zeros
+    if (used == 1) finish(i, L[k], a[k]);
+    else if (!kJoin) write_part<D>(part, (((int64_t)s * C.kv_heads + g) * kDecodeRows + r) * splits + z, d, M[k], L[k], a[k]);
+  }
+  if (kJoin && used > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    __syncthreads();  // the warps' o have been read: the CTA's own goes over them, row by row as in a part
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) a[e] *= inv;
-      store8(out + (int64_t)t * out_ld + (int64_t)h * D + d, a);
+    for (int k = 0; k < kItems; ++k) {
+      const int i = threadIdx.x + k * 32 * kDecodeWarps;
+      if (i < items) write_part<D>(so, i / (D / kPer), i % (D / kPer) * kPer, M[k], L[k], a[k]);
     }
+    cl.sync();
+    for (int i = threadIdx.x + 32 * kDecodeWarps * z; i < items; i += 32 * kDecodeWarps * used) {
+      const int r = i / (D / kPer), d = i % (D / kPer) * kPer;
+      float2 ml[kJoinSplits];
+      float m = -INFINITY, l = 0.0f, x[kPer] = {};
+#pragma unroll
+      for (int y = 0; y < kJoinSplits; ++y) {
+        ml[y] = y < used ? *reinterpret_cast<const float2*>(cl.map_shared_rank(so, y) + r * (D + 8) + D)
+                         : make_float2(-INFINITY, 0.0f);
+        m = fmaxf(m, ml[y].x);
+      }
+#pragma unroll
+      for (int y = 0; y < kJoinSplits; ++y) {
+        if (y >= used) break;
+        const float f = ml[y].x == -INFINITY ? 0.0f : exp2_approx(ml[y].x - m);
+        float v[kPer];
+        load8(cl.map_shared_rank(so, y) + r * (D + 8) + d, v);
+        l = fmaf(ml[y].y, f, l);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) x[e] = fmaf(v[e], f, x[e]);
+      }
+      finish(i, l, x);
+    }
+    cl.sync();  // nobody's shared memory goes before it has been read
   }
   // launched beside the chunk form: this grid ends after it, so that whoever waits for this one
   // has waited for both

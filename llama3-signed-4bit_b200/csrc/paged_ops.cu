@@ -131,17 +131,24 @@ static Cache cache_of(const llama_paged_kv_t* kv) {
 // after its griddepcontrol.wait.
 template <typename... KArgs, typename... Args>
 static void launch(bool early, void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
-                   Args... args) {
+                   int cluster, Args... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute at[2];
   cfg.attrs = at;
-  cfg.numAttrs = early ? 1 : 0;
+  if (early) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
@@ -159,7 +166,7 @@ const char* append_rows(const llama_paged_kv_t* kv, const void* qkv, int type, i
     using Kv = decltype(c);
     using Q = decltype(q);
     auto* fn = D == 64 ? k_paged_append<In, Kv, Q, 64> : k_paged_append<In, Kv, Q, 128>;
-    launch(chained, fn, grid, 256, 0, st, C, static_cast<const In*>(qkv), ld, planes, plane_stride, rows, heads, pos, seq,
+    launch(chained, fn, grid, 256, 0, st, 1, C, static_cast<const In*>(qkv), ld, planes, plane_stride, rows, heads, pos, seq,
            rope_cos, rope_sin, n_pos, static_cast<Q*>(q_out), q_ld);
   };
   auto by_type = [&](auto c) {
@@ -174,12 +181,14 @@ const char* append_rows(const llama_paged_kv_t* kv, const void* qkv, int type, i
 }
 
 constexpr int kSms = 148;  // the workspace's size must not need a device
-constexpr int kDecodeCtas = 8 * kSms, kChunkItems = 4 * kSms;  // bounds of what splitting makes
+constexpr int kSmSharedBytes = 227 * 1024;  // that an SM's CTAs can have together
+constexpr int kChunkItems = 4 * kSms;  // bounds what splitting makes
+constexpr double kKeysRoot = 0.9;
 
 // How a call is cut: which kernels run, and their key splits.
 struct Plan {
   SplitPlan sp{};
-  bool decode = false, chunk = false;
+  bool decode = false, chunk = false, join = false;  // join: decode splits are joined by clusters
   size_t bytes = 0;
 };
 static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, int max_kv) {
@@ -191,11 +200,24 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   P.decode = !P.chunk || (kv->seqs > 1 && rows < (int64_t)kv->seqs * max_q && G <= kDecodeRows);
   P.sp.small_rows = P.decode ? kDecodeRows : 0;
   const int64_t units = (int64_t)std::min(kv->seqs, std::max(rows, 1)) * kv->kv_heads;
-  // decode: about eight CTAs for every SM where the keys allow, of 64 keys (one slice for each warp) at least
-  int64_t per = (units * keys + kDecodeCtas - 1) / kDecodeCtas;
-  per = std::max<int64_t>(64, (per + 63) / 64 * 64);
+  // decode: a CTA's start and end cost as much as some hundred keys, and the last CTAs of many short ones
+  // end closer together, so keys per CTA and CTAs grow alike, as the root of the call's keys.  At 0.9 of
+  // it 64 x 2048 takes 35.8 us (0.7 35.5, 1.4 37.6), 128 x 8192 333 us (332, 340), 1 x 4096 8.4 us (7.9,
+  // 9.9), 8 x 2048 with heads of 128 19.0 us (17.3, 14.6); 128 keys are two slices for each warp.
+  int64_t per = (int64_t)std::ceil(kKeysRoot * std::sqrt((double)units * keys));
+  per = std::max<int64_t>(128, (per + 63) / 64 * 64);
+  int64_t parts = (keys + per - 1) / per;
+  // A cluster of up to eight CTAs joins a sequence's splits where all CTAs are resident at once: no second
+  // launch and no parts in memory (1 x 700 9.2 -> 6.2 us, 16 x 1000 11.4 -> 9.8 us).  Beyond that the
+  // clusters, which hold their shared memory until their last CTA is done, cost more (64 x 2048 37 -> 43 us).
+  const int64_t resident = (int64_t)kSms * (kSmSharedBytes / (kv->head_dim == 64 ? DecodeGeo<64>::kSmem : DecodeGeo<128>::kSmem));
+  if (parts > kJoinSplits && parts <= 2 * kJoinSplits && units * kJoinSplits <= resident) {
+    per = (keys + kJoinSplits * 64 - 1) / (kJoinSplits * 64) * 64;
+    parts = (keys + per - 1) / per;
+  }
+  P.join = P.decode && parts > 1 && parts <= kJoinSplits && units * parts <= resident;
   P.sp.per[0] = (int)per;
-  P.sp.splits[0] = P.decode ? (int)((keys + per - 1) / per) : 1;
+  P.sp.splits[0] = P.decode ? (int)parts : 1;
   // chunk: one CTA per SM; as many splits as make the estimate smallest: the busiest SM's key tiles,
   // three more for each of its items, and the parts' way through memory, of which about 8 MB pass in the
   // 1.9 us of a key tile.  512 tokens over 32768 keys (8 x 8 items): 2 splits 251 us, 9 (which would
@@ -218,7 +240,7 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
       }
     }
   }
-  const int64_t n0 = P.sp.splits[0] > 1 ? (int64_t)kv->seqs * kv->kv_heads * kDecodeRows * P.sp.splits[0] : 0;
+  const int64_t n0 = P.sp.splits[0] > 1 && !P.join ? (int64_t)kv->seqs * kv->kv_heads * kDecodeRows * P.sp.splits[0] : 0;
   const int64_t n1 = P.sp.splits[1] > 1 ? (int64_t)rows * heads * P.sp.splits[1] : 0;
   P.sp.part1 = n0;
   P.bytes = (size_t)(n0 + n1) * (kv->head_dim + 8) * sizeof(float);
@@ -288,30 +310,41 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
     if (!query_map(&mq, kv, q, q_ld, heads, rows) || !pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v))
       return "tensor maps could not be made";
     if (!allow_smem(k_paged_chunk<T, O, D>, ChunkGeo<D>::kSmem, dev)) return "shared memory could not be set";
-    launch(chained, k_paged_chunk<T, O, D>, (unsigned)items, kChunkThreads, ChunkGeo<D>::kSmem, st,
+    launch(chained, k_paged_chunk<T, O, D>, (unsigned)items, kChunkThreads, ChunkGeo<D>::kSmem, st, 1,
            mq, mk, mv, C, heads, cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], ot, out_ld,
            part + P.sp.part1 * (D + 8), waits);
   }
   if (P.decode) {
     const int64_t grid = (int64_t)C.seqs * C.kv_heads * P.sp.splits[0];
     if (grid > 0x7fffffff) return "too many sequences";
-    if (!allow_smem(k_paged_decode<T, O, D>, DecodeGeo<D>::kSmem, dev)) return "shared memory could not be set";
-    launch(P.chunk || chained, k_paged_decode<T, O, D>, (unsigned)grid, 32 * kDecodeWarps, DecodeGeo<D>::kSmem, st, C, qt, q_ld,
-           heads, cu_q, kv_len, rows, scale * 1.44269504f, P.sp.per[0], P.sp.splits[0], P.chunk ? 1 : 0, ot, out_ld, part);
+    auto* fn = P.join ? k_paged_decode<T, O, D, true> : k_paged_decode<T, O, D, false>;
+    if (!allow_smem(fn, DecodeGeo<D>::kSmem, dev)) return "shared memory could not be set";
+    launch(P.chunk || chained, fn, (unsigned)grid, 32 * kDecodeWarps, DecodeGeo<D>::kSmem, st, P.join ? P.sp.splits[0] : 1, C,
+           qt, q_ld, heads, cu_q, kv_len, rows, scale * 1.44269504f, P.sp.per[0], P.sp.splits[0], P.chunk ? 1 : 0, ot, out_ld,
+           part);
   }
-  if (P.sp.splits[0] > 1 || P.sp.splits[1] > 1) {
-    const int64_t grid = ((int64_t)rows * heads * (D / 8) + 127) / 128;
+  if ((P.sp.splits[0] > 1 && !P.join) || P.sp.splits[1] > 1) {
+    // a group of threads for every kCombineRun splits, as far as a block goes
+    const int most = std::max(P.join ? 1 : P.sp.splits[0], P.sp.splits[1]);
+    int groups_log2 = 0;
+    while (most > kCombineRun << groups_log2 && D / 8 << groups_log2 < kCombineThreads) ++groups_log2;
+    const int64_t grid = (((int64_t)rows * heads * (D / 8) << groups_log2) + kCombineThreads - 1) / kCombineThreads;
     if (grid > 0x7fffffff) return "too many rows";
-    launch(true, k_paged_combine<O, D>, (unsigned)grid, 128, 0, st, C, heads, cu_q, kv_len, rows, P.sp, part, ot, out_ld);
+    SplitPlan sp = P.sp;
+    if (P.join) sp.splits[0] = 1;  // those have been joined
+    launch(true, k_paged_combine<O, D>, (unsigned)grid, kCombineThreads, 0, st, 1, C, heads, cu_q, kv_len, rows, sp,
+           groups_log2, part, ot, out_ld);
   }
   return nullptr;
 }
 
-// No plan for seqs <= rows needs more: a decode tile is split only while there are fewer than
-// kDecodeCtas (sequence, kv head) pairs, into at most kDecodeCtas + that many splits in all; chunks into
-// at most kChunkItems (item, split) pairs of two row tiles.
-size_t attention_bytes_max(int head_dim) {
-  return ((size_t)kDecodeRows * 2 * kDecodeCtas + (size_t)2 * kTileRows * kChunkItems) * (head_dim + 8) * sizeof(float);
+// A call of W keys over all its (sequence, kv head) pairs has at most W / (kKeysRoot sqrt(W)) decode
+// splits and one more for each pair; chunks make at most kChunkItems (item, split) pairs of two row
+// tiles.
+size_t attention_bytes_max(int head_dim, int kv_heads, int seqs, int max_kv) {
+  const double units = (double)seqs * kv_heads;
+  const size_t splits = (size_t)(std::sqrt(units * max_kv) / kKeysRoot + units) + 1;
+  return (kDecodeRows * splits + (size_t)2 * kTileRows * kChunkItems) * (head_dim + 8) * sizeof(float);
 }
 
 const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, int64_t q_ld, int heads,
