@@ -217,37 +217,72 @@ struct Item {
   int k_lo;          // first key of the split
   int nk[2];         // key tiles that the row tiles see
 };
-// Item w of the launch (kv heads fastest, then splits, then the row tiles from the last sequence's last),
-// found by a whole warp; the result is the same in every lane.
+// Items of a sequence (two row tiles each), and those of them that see more than `keys` keys (all of them
+// for keys < 0): item j's last token is the ((2 j + 1) / parts + 1) tokens-th, so they are the last ones.
+__device__ __forceinline__ int items_of(const Span& sp, const RowTiles& T, int small_rows) {
+  return sp.n <= 0 || sp.n * T.G <= small_rows ? 0 : ((sp.n + T.tokens - 1) / T.tokens * T.parts + 1) / 2;
+}
+__device__ __forceinline__ int items_above(const Span& sp, const RowTiles& T, int items, int keys) {
+  const int y = keys - (sp.len - sp.n);
+  return keys < 0 || y < 0 ? items : y >= sp.n ? 0 : items - min(items, T.parts * (y / T.tokens) / 2);
+}
+// Item w of the launch: kv heads fastest, then splits, then the pairs of row tiles.  longest (at most 32
+// sequences): the pairs in order of the key tiles they see, the most first, so that the last items are
+// short ones; otherwise the sequences from the last to the first, each from its last pair to its first,
+// which keeps a sequence's keys in L2 while they are used.  Found by
+// a whole warp; the result is the same in every lane.
 __device__ __forceinline__ Item find_item(const Cache& C, const int32_t* cu_q, const int32_t* kv_len, int rows,
-                                          const RowTiles& T, int small_rows, int per, int splits, int total, int w) {
+                                          const RowTiles& T, int small_rows, int per, int splits, int total, int longest,
+                                          int w) {
   const int lane = threadIdx.x & 31;
   Item it;
   it.seq = -1;
   if (w < 0) return it;
   it.g = w % C.kv_heads;
   it.z = (w / C.kv_heads) % splits;
-  const int want = total - 1 - w / C.kv_heads / splits;
+  int want = w / C.kv_heads / splits;
+  if (want >= total) return it;
   int before = 0, local = 0;
-  for (int s0 = 0; s0 < C.seqs && it.seq < 0 && want >= 0; s0 += 32) {
-    int mine = 0;
-    if (s0 + lane < C.seqs) {
-      const int n = max(span_of(C, cu_q, kv_len, s0 + lane, rows).n, 0);
-      mine = n * T.G <= small_rows ? 0 : ((n + T.tokens - 1) / T.tokens * T.parts + 1) / 2;
+  if (longest) {
+    Span sp{0, 0, 0};
+    if (lane < C.seqs) sp = span_of(C, cu_q, kv_len, lane, rows);
+    const int items = items_of(sp, T, small_rows);
+    auto above = [&](int tiles) { return items_above(sp, T, items, tiles * kTileKeys); };
+    // the item sees more than lo key tiles and at most hi
+    int lo = -1, hi = ((int)__reduce_max_sync(0xffffffffu, (unsigned)sp.len) + kTileKeys - 1) / kTileKeys;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int)__reduce_add_sync(0xffffffffu, (unsigned)above(mid)) > want) lo = mid;
+      else hi = mid;
     }
-    int inc = mine;
+    const int longer = above(hi), here = above(lo);
+    want -= (int)__reduce_add_sync(0xffffffffu, (unsigned)longer);
+    int inc = here - longer;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > want);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      it.seq = s0 + l;
-      local = want - before - __shfl_sync(0xffffffffu, inc - mine, l);
+    it.seq = __ffs(__ballot_sync(0xffffffffu, inc > want)) - 1;
+    local = __shfl_sync(0xffffffffu, items - here + want - (inc - (here - longer)), max(it.seq, 0));
+  } else {
+    want = total - 1 - want;
+    for (int s0 = 0; s0 < C.seqs && it.seq < 0; s0 += 32) {
+      const int mine = s0 + lane < C.seqs ? items_of(span_of(C, cu_q, kv_len, s0 + lane, rows), T, small_rows) : 0;
+      int inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > want);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        it.seq = s0 + l;
+        local = want - before - __shfl_sync(0xffffffffu, inc - mine, l);
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
     }
-    before += __shfl_sync(0xffffffffu, inc, 31);
   }
   if (it.seq < 0) return it;
   const Span sp = span_of(C, cu_q, kv_len, it.seq, rows);
@@ -273,10 +308,7 @@ __device__ __forceinline__ int count_items(const Cache& C, const int32_t* cu_q, 
                                            const RowTiles& T, int small_rows) {
   const int lane = threadIdx.x & 31;
   int total = 0;
-  for (int s = lane; s < C.seqs; s += 32) {
-    const int n = max(span_of(C, cu_q, kv_len, s, rows).n, 0);
-    if (n * T.G > small_rows) total += ((n + T.tokens - 1) / T.tokens * T.parts + 1) / 2;
-  }
+  for (int s = lane; s < C.seqs; s += 32) total += items_of(span_of(C, cu_q, kv_len, s, rows), T, small_rows);
   return (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
 }
 
@@ -305,7 +337,7 @@ template <typename T, typename O, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     k_paged_chunk(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, Cache C, int heads, const int32_t* __restrict__ cu_q,
-                  const int32_t* __restrict__ kv_len, int rows, float scale, int small_rows, int per, int splits,
+                  const int32_t* __restrict__ kv_len, int rows, float scale, int small_rows, int per, int splits, int longest,
                   O* __restrict__ out, int64_t out_ld, float* __restrict__ part, Waits W) {
   using Geo = ChunkGeo<D>;
   constexpr int kSt = Geo::kStages, kQb = Geo::kQBufs;
@@ -376,7 +408,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         Item it;
         if (kv == 0) {
           do {  // past the last item the launch has CTAs without work
-            it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, w);
+            it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, longest, w);
             if (it.seq < 0 && w >= 0) {
               steal();
               stolen();
@@ -786,7 +818,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (s_abort && warp < 8) {
     const int i = warp >> 2, total = count_items(C, cu_q, kv_len, rows, R, small_rows);
     for (int k = item; k < s_claims; ++k) {
-      const Item it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, s_claimed[k & 3]);
+      const Item it = find_item(C, cu_q, kv_len, rows, R, small_rows, per, splits, total, longest, s_claimed[k & 3]);
       if (it.seq < 0) continue;
       const Row row = row_of(it, R, i, tid & 127);
       if (!row.live || it.z >= it.used) continue;

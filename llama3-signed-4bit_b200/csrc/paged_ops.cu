@@ -184,11 +184,13 @@ constexpr int kSms = 148;  // the workspace's size must not need a device
 constexpr int kSmSharedBytes = 227 * 1024;  // that an SM's CTAs can have together
 constexpr int kChunkItems = 4 * kSms;  // bounds what splitting makes
 constexpr double kKeysRoot = 0.9;
+constexpr int kLongestBytes = 640 << 20;  // of keys and values when all have max_kv of them; L2 has 126 MB
 
 // How a call is cut: which kernels run, and their key splits.
 struct Plan {
   SplitPlan sp{};
   bool decode = false, chunk = false, join = false;  // join: decode splits are joined by clusters
+  bool longest = false;  // chunk items in order of their keys
   size_t bytes = 0;
 };
 static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, int max_kv) {
@@ -239,6 +241,12 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
         P.sp.splits[1] = (int)((keys + p1 - 1) / p1);
       }
     }
+    // The longest items first where SMs take several: 8 ragged chunks of 611 over 3001 104 -> 94 us, 32 of
+    // 256 over 4096 252 -> 227 us.  Not where the sequences' keys are far beyond L2, since each item
+    // then brings its own from memory: 16 equal chunks of 1024 over 16384 take 3.53 -> 3.82 ms so.  Among
+    // more than 32 sequences (a lane each) an item is short against the whole.
+    P.longest = kv->seqs > 1 && kv->seqs <= 32 && items * P.sp.splits[1] > kSms &&
+                units * keys * kv->head_dim * 4 <= (int64_t)kLongestBytes;
   }
   const int64_t n0 = P.sp.splits[0] > 1 && !P.join ? (int64_t)kv->seqs * kv->kv_heads * kDecodeRows * P.sp.splits[0] : 0;
   const int64_t n1 = P.sp.splits[1] > 1 ? (int64_t)rows * heads * P.sp.splits[1] : 0;
@@ -311,7 +319,7 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
       return "tensor maps could not be made";
     if (!allow_smem(k_paged_chunk<T, O, D>, ChunkGeo<D>::kSmem, dev)) return "shared memory could not be set";
     launch(chained, k_paged_chunk<T, O, D>, (unsigned)items, kChunkThreads, ChunkGeo<D>::kSmem, st, 1,
-           mq, mk, mv, C, heads, cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], ot, out_ld,
+           mq, mk, mv, C, heads, cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], P.longest ? 1 : 0, ot, out_ld,
            part + P.sp.part1 * (D + 8), waits);
   }
   if (P.decode) {

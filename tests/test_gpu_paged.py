@@ -155,6 +155,18 @@ SHAPES = [
     ("f16", 64, 12, 2, 32, [33, 7, 100, 200, 1, 37, 64, 21, 43, 90, 11, 130, 17, 300] * 6,
      [33, 5, 4000, 201, 9, 37, 64, 400, 44, 3, 1100, 130, 18, 311] * 6),
     ("f16", 128, 200, 1, 16, [1, 2, 3] * 40, [200, 17, 130] * 40),
+    # several items for every SM of at most 32 sequences, in order of their keys: equal ones, rows without keys
+    ("f16", 64, 32, 8, 16, [700, 1, 0, 500, 37, 130, 260], [700, 900, 10, 333, 1500, 129, 0]),
+    ("bf16", 128, 56, 8, 32, [200, 90, 1, 36, 301, 37, 5, 250, 18], [1500, 90, 700, 36, 301, 2000, 5, 251, 18]),
+    ("f16", 128, 300, 2, 16, [40, 3, 60], [50, 3, 900]),
+    ("bf16", 64, 64, 8, 16, [33] * 32, [600] * 32),
+    # single tokens: splits joined by a cluster, of which sequences use all, some, one or none
+    ("bf16", 128, 32, 8, 64, [1, 2, 0, 1], [1000, 129, 70, 1]),
+    ("f16", 64, 16, 16, 16, [1, 1, 1, 4], [700, 0, 300, 4]),
+    # more splits than a cluster has: joined by groups of threads, a few and many
+    ("f16", 64, 8, 8, 16, [1], [20000]),
+    ("bf16", 128, 24, 2, 16, [1, 1], [11000, 900]),
+    ("f16", 64, 32, 8, 32, [1, 2] * 20, [3000, 70, 900, 2, 1500, 17, 640, 2048, 1, 63] * 4),
 ]
 
 
