@@ -113,7 +113,8 @@ llama_engine_t llama_engine_create_ex(const char* model_path, int device, int ma
  * anything.  Keys, values and rotated queries are rounded to cache_type, so logits differ from the
  * fp32 cache's by that rounding.  Needs the tensor-core batched path; every step runs on it,
  * forward_token and generate_greedy as steps of one row.  A position that was never fed holds no key
- * (positions of a page that was given out for a neighbour hold stale ones: feed a sequence in order).
+ * (positions of a page that was given out for a neighbour hold zeros, or what a released sequence left
+ * there: feed a sequence in order).
  * profile_phase is not available.  NULL on failure. */
 llama_engine_t llama_engine_create_paged(const char* model_path, int device, int max_batch, int max_seq_len,
                                          int num_pages, int page_size, int cache_type);

@@ -1409,6 +1409,8 @@ static bool init_device(Engine* E, const uint8_t* base, const ParsedFile& P) {
     const size_t pool = (size_t)E->layers * E->num_pages * E->page_size * E->kv_dim * 2;
     LE_CK(cudaMalloc(&E->pool_k, pool));
     LE_CK(cudaMalloc(&E->pool_v, pool));
+    LE_CK(cudaMemsetAsync(E->pool_k, 0, pool, E->stream));  // rows that are never fed are finite
+    LE_CK(cudaMemsetAsync(E->pool_v, 0, pool, E->stream));
     E->page_width = (E->max_seq + E->page_size - 1) / E->page_size;
     const size_t entries = (size_t)E->max_batch * E->page_width;
     LE_CK(cudaMalloc(&E->d_table, entries * 4));

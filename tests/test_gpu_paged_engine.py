@@ -62,6 +62,20 @@ def test_prefill_decode_and_scores_match_the_flat_engine(pkg, bindings, small_mo
         eng.close()
 
 
+def test_positions_that_were_skipped_within_a_page(pkg, bindings, small_model):
+    """Rows of a fresh page that are never fed count as keys of zeros, as in the flat engine."""
+    flat = pkg.LlamaEngine(str(small_model), bindings, device=0, max_batch=1, max_seq_len=64)
+    eng = pkg.LlamaEngine(str(small_model), bindings, device=0, max_batch=1, max_seq_len=64, num_pages=2, page_size=32)
+    try:
+        for e in (flat, eng):
+            e.forward_token(77, 20, True)
+        assert near(eng.get_logits(), flat.get_logits(), 1)
+        assert eng.free_pages == 1
+    finally:
+        flat.close()
+        eng.close()
+
+
 def test_batched_rows_of_many_slots(pkg, bindings, small_model):
     """Rows in any order: single positions, several positions of a slot in one call, slots interleaved."""
     flat = pkg.LlamaEngine(str(small_model), bindings, device=0, max_batch=8, max_seq_len=256)
