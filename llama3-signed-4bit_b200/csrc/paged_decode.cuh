@@ -10,17 +10,17 @@
 //   * The G heads x n tokens that share a kv head are the 16 rows of one mma.sync tile, so a key is
 //     read once for all of them.  (The 5th-generation tensor cores would compute 128 rows of which
 //     at most 16 exist; the product is a few per cent of the time either way.)
-//   * The keys are cut into splits of `per` keys, one CTA each, and a CTA's four warps take
+//   * The keys are cut into splits, one CTA each, and a CTA's four warps take
 //     16-key slices of the split in turn.  A slice lies within one page (pages are multiples of
 //     16 rows), so it has one table entry, and a page id out of range drops the slice.
 //   * Every warp streams its slices through its own ring in shared memory (cp.async, 16-byte chunks
 //     XOR-swizzled by row so that ldmatrix is free of conflicts): no barrier between the warps until
 //     they merge their (m, l, o) at the end.  Rows past the length are zero-filled: what stale
 //     memory holds there meets weights of 0 and must not be NaN.
-//   * Up to eight splits of a sequence and kv head are one thread-block cluster, whose CTAs join their
-//     unnormalised (m, l, o) through distributed shared memory.  More of them (few sequences with many
-//     keys) write them in fp32 and k_paged_combine joins them.  A sequence that fits one split is
-//     written at once.
+//   * The splits of a sequence and kv head are one thread-block cluster where that suits the call: it cuts
+//     the sequence evenly and joins the CTAs' unnormalised (m, l, o) through distributed shared
+//     memory.  Otherwise they are written in fp32 and k_paged_combine joins them.  A sequence of one
+//     split is written at once.
 // The weights are rounded to the cache's type for the product with v (the type its v has), the sum
 // l takes them unrounded in fp32.
 //
@@ -43,7 +43,8 @@ namespace paged {
 
 constexpr int kSlice = 16;        // keys a warp takes at a time
 constexpr int kDecodeWarps = 4;
-constexpr int kJoinSplits = 8;    // splits that a cluster joins
+constexpr int kJoinSplits = 8;    // splits that a cluster joins at most
+constexpr int kJoinKeys = 128;    // keys of such a split at least: two slices for each warp
 template <int D> struct DecodeGeo {
   static constexpr int kStages = D == 64 ? 4 : 3;              // slices in flight per warp
   static constexpr int kSliceBytes = kSlice * D * 2;           // K (or V) of a slice
@@ -76,8 +77,8 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, 
 
 // Grid: seqs x splits x kv_heads, kv heads fastest (their CTAs read neighbouring bytes of the same
 // rows); kJoin: seqs x kv_heads x splits, the splits of a pair a cluster.  per: keys of a split, a
-// multiple of 64; the last split takes all keys behind it.  beside: launched while the chunk form of
-// the same call runs, whose inputs are complete.
+// multiple of 64 (kJoin: of the sequence's own length); the last split takes all keys behind it.
+// beside: launched while the chunk form of the same call runs, whose inputs are complete.
 template <typename T, typename O, int D, bool kJoin>
 __global__ void __launch_bounds__(32 * kDecodeWarps)
     k_paged_decode(Cache C, const T* __restrict__ q, int64_t q_ld, int heads, const int32_t* __restrict__ cu_q,
@@ -95,6 +96,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
   const int s = blockIdx.x / C.kv_heads / splits;
   const Span sp = span_of(C, cu_q, kv_len, s, rows);
   const int G = heads / C.kv_heads, R = sp.n * G;
+  if (kJoin) per = max(kJoinKeys, ((sp.len + splits - 1) / splits + 63) & ~63);
   const int used = splits_of(sp.len, per, splits);
   namespace cg = cooperative_groups;
   if (sp.n <= 0 || R > kDecodeRows || z >= used) {  // nothing to do, or the chunk form's

@@ -214,15 +214,15 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   int64_t per = (int64_t)std::ceil(kKeysRoot * std::sqrt((double)units * keys));
   per = std::min(std::max<int64_t>(128, (per + 63) / 64 * 64), std::max<int64_t>(128, (keys + 63) / 64 * 64));
   int64_t parts = (keys + per - 1) / per;
-  // A cluster of up to eight CTAs joins a sequence's splits where all CTAs are resident at once: no second
-  // launch and no parts in memory (1 x 700 9.2 -> 6.2 us, 16 x 1000 11.4 -> 9.8 us).  Beyond that the
-  // clusters, which hold their shared memory until their last CTA is done, cost more (64 x 2048 37 -> 43 us).
+  // Where all CTAs can be resident at once, a cluster of them takes each pair and joins its splits: no second
+  // launch, no parts in memory, and every sequence cut evenly (1 x 700 9.2 -> 6.1 us, 16 x 2048 13.6 -> 12.7,
+  // 8 x 2048 with heads of 128 19.0 -> 15.0).  Beyond that clusters wait for one another's shared memory (64 x
+  // 2048, clusters of 4: 36 -> 44 us), and pairs whose keys are worth many more CTAs than a cluster has
+  // are faster without (1 x 32768, clusters of 8: 18.5 -> 35 us).
   const int64_t resident = (int64_t)kSms * (kSmSharedBytes / (kv->head_dim == 64 ? DecodeGeo<64>::kSmem : DecodeGeo<128>::kSmem));
-  if (parts > kJoinSplits && parts <= 2 * kJoinSplits && units * kJoinSplits <= resident) {
-    per = (keys + kJoinSplits * 64 - 1) / (kJoinSplits * 64) * 64;
-    parts = (keys + per - 1) / per;
-  }
-  P.join = P.decode && parts > 1 && parts <= kJoinSplits && units * parts <= resident;
+  const int64_t joined = std::min({(int64_t)kJoinSplits, resident / units, (keys + kJoinKeys - 1) / kJoinKeys});
+  P.join = P.decode && joined > 1 && parts <= 2 * kJoinSplits;
+  if (P.join) parts = joined;
   P.sp.per[0] = (int)per;
   P.sp.splits[0] = P.decode ? (int)parts : 1;
   // chunk: one CTA per SM; as many splits as make the estimate smallest: the busiest SM's key tiles,
