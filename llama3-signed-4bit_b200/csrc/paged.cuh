@@ -140,40 +140,55 @@ struct SplitPlan {
 };
 
 // out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the splits of a (row, head), M = max m_z;
-// rows whose sequence has one split were written already.  D / 8 << groups_log2 threads per (row,
-// head), 8 outputs each: a group of D / 8 takes every groups-th split with a running (M, L, o), and
-// the groups join through shared memory.  A thread's loads follow one another's addresses only, so
-// kCombineRun splits are in flight at a time.  Against one group that walks all splits: attention of one
-// token over 32768 keys (48 splits) 46 -> 18.5 us, over 4096 23 -> 8.4 us.
+// rows whose sequence has one split were written already.  The first blocks0 blocks take the rows of
+// decode tiles (tile_rows of each sequence and kv head), the others all rows, of which those of chunks are
+// theirs.  D / 8 << groups_log2 threads per (row, head), 8 outputs each: a group of D / 8 takes every
+// groups-th split with a running (M, L, o), and the groups join through shared memory.  A thread's loads
+// follow one another's addresses only, so kCombineRun splits are in flight at a time.  Against one group
+// that walks all splits: attention of one token over 32768 keys (37 splits) 46 -> 18.5 us, over 4096
+// 23 -> 8.4 us.  Against looking every row of the call up: 32 chunks of 256 over 4096, with a single
+// token and an idle sequence among them, 279 -> 216 us.
 constexpr int kCombineThreads = 128, kCombineRun = 4;
 template <typename O, int D>
 __global__ void __launch_bounds__(kCombineThreads)
     k_paged_combine(Cache C, int heads, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ kv_len, int rows,
-                    SplitPlan P, int groups_log2, const float* __restrict__ part, O* __restrict__ out, int64_t out_ld) {
+                    SplitPlan P, int blocks0, int tile_rows, int groups_log2, const float* __restrict__ part,
+                    O* __restrict__ out, int64_t out_ld) {
   grid_dep_wait();  // the parts come from the kernel before
   constexpr int kRuns = D / 8;
   __shared__ __align__(16) float s_a[kCombineThreads][8];
   __shared__ float2 s_ml[kCombineThreads];
   const int groups = 1 << groups_log2, mine = threadIdx.x % kRuns, grp = threadIdx.x / kRuns % groups;
-  const int64_t rh = ((int64_t)blockIdx.x * kCombineThreads + threadIdx.x) / (kRuns * groups);
-  const int d = mine * 8, t = (int)(rh / heads), h = (int)(rh % heads);
-  int used = 0;  // splits to join: none where the row is nobody's, or has been written
+  const int d = mine * 8, G = heads / C.kv_heads;
+  int used = 0, t = 0, h = 0;  // splits to join: none where the row is nobody's, or has been written
   const float* p = part;
-  if (t < rows) {
-    int lo = 0, hi = C.seqs;  // sequence of row t: the first whose end lies behind it
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (cu_q[mid + 1] <= t) lo = mid + 1;
-      else hi = mid;
+  if ((int)blockIdx.x < blocks0) {
+    const int64_t i = ((int64_t)blockIdx.x * kCombineThreads + threadIdx.x) / (kRuns * groups);
+    const int r = (int)(i % tile_rows), g = (int)(i / tile_rows % C.kv_heads);
+    const int64_t s = i / tile_rows / C.kv_heads;
+    if (s < C.seqs) {
+      const Span sp = span_of(C, cu_q, kv_len, (int)s, rows);
+      t = sp.first + r / G;
+      h = g * G + r % G;
+      if (r < sp.n * G && sp.n * G <= P.small_rows) used = splits_of(sp.len, P.per[0], P.splits[0]);
+      if (used > 1) p += ((s * C.kv_heads + g) * kDecodeRows + r) * P.splits[0] * (D + 8);
     }
-    if (lo < C.seqs) {
-      const Span sp = span_of(C, cu_q, kv_len, lo, rows);
-      const int G = heads / C.kv_heads, kind = sp.n * G <= P.small_rows ? 0 : 1;
-      const int S = P.splits[kind];
-      used = t < sp.first ? 0 : splits_of(sp.len, P.per[kind], S);
-      if (used > 1)
-        p += (kind ? P.part1 + rh * S : (((int64_t)lo * C.kv_heads + h / G) * kDecodeRows + (t - sp.first) * G + h % G) * S) *
-             (D + 8);
+  } else {
+    const int64_t rh = ((int64_t)(blockIdx.x - blocks0) * kCombineThreads + threadIdx.x) / (kRuns * groups);
+    t = (int)(rh / heads);
+    h = (int)(rh % heads);
+    if (t < rows) {
+      int lo = 0, hi = C.seqs;  // sequence of row t: the first whose end lies behind it
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cu_q[mid + 1] <= t) lo = mid + 1;
+        else hi = mid;
+      }
+      if (lo < C.seqs) {
+        const Span sp = span_of(C, cu_q, kv_len, lo, rows);
+        if (t >= sp.first && sp.n * G > P.small_rows) used = splits_of(sp.len, P.per[1], P.splits[1]);
+        if (used > 1) p += (P.part1 + rh * P.splits[1]) * (D + 8);
+      }
     }
   }
   float M = -INFINITY, L = 0.0f, a[8] = {};

@@ -209,8 +209,8 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   const int64_t units = (int64_t)std::min(kv->seqs, std::max(rows, 1)) * kv->kv_heads;
   // decode: a CTA's start and end cost as much as some hundred keys, and the last CTAs of many short ones
   // end closer together, so keys per CTA and CTAs grow alike, as the root of the call's keys.  At 0.9 of
-  // it 64 x 2048 takes 35.8 us (0.7 35.5, 1.4 37.6), 128 x 8192 333 us (332, 340), 1 x 4096 8.4 us (7.9,
-  // 9.9), 8 x 2048 with heads of 128 19.0 us (17.3, 14.6); 128 keys are two slices for each warp.
+  // it (with a combine) 64 x 2048 takes 35.8 us (0.7 35.5, 1.4 37.6), 128 x 8192 333 us (332, 340), 1 x 4096
+  // 8.4 us (7.9, 9.9); 128 keys are two slices for each warp.
   int64_t per = (int64_t)std::ceil(kKeysRoot * std::sqrt((double)units * keys));
   per = std::min(std::max<int64_t>(128, (per + 63) / 64 * 64), std::max<int64_t>(128, (keys + 63) / 64 * 64));
   int64_t parts = (keys + per - 1) / per;
@@ -246,10 +246,10 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
         P.sp.splits[1] = (int)((keys + p1 - 1) / p1);
       }
     }
-    // The longest items first where SMs take several: 8 ragged chunks of 611 over 3001 104 -> 94 us, 32 of
-    // 256 over 4096 252 -> 227 us.  Not where the sequences' keys are far beyond L2, since each item
-    // then brings its own from memory: 16 equal chunks of 1024 over 16384 take 3.53 -> 3.82 ms so.  Among
-    // more than 32 sequences (a lane each) an item is short against the whole.
+    // The longest items first where SMs take several: 8 ragged chunks of 611 over 3001 104 -> 94 us.  Not
+    // where the sequences' keys are far beyond L2, since each item then brings its own from memory: 16
+    // equal chunks of 1024 over 16384 take 3.53 -> 3.82 ms so.  Up to 32 sequences, a lane each; with four
+    // for each lane every look-up takes longer than the order gains (8 x 2048 248 -> 250 us).
     P.longest = kv->seqs > 1 && kv->seqs <= 32 && items * P.sp.splits[1] > kSms &&
                 units * keys * kv->head_dim * 4 <= (int64_t)kLongestBytes;
   }
@@ -309,15 +309,15 @@ static uint32_t* error_word(int dev) {
 
 template <typename T, typename O, int D>
 static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Cache& C, int dev, const void* q, int64_t q_ld, int heads,
-                             const int32_t* cu_q, const int32_t* kv_len, int rows, float scale, void* out,
+                             const int32_t* cu_q, const int32_t* kv_len, int rows, int max_q, float scale, void* out,
                              int64_t out_ld, float* part, const Waits& waits, cudaStream_t st, bool chained) {
   const T* qt = static_cast<const T*>(q);
   O* ot = static_cast<O*>(out);
   if (P.chunk) {
     // two row tiles an item, every sequence's last one perhaps half empty
     const RowTiles R = row_tiles(heads / C.kv_heads);
-    const int64_t tiles = ((int64_t)rows / R.tokens + std::min(C.seqs, rows)) * R.parts;
-    const int64_t items = (tiles / 2 + std::min(C.seqs, rows)) * C.kv_heads * P.sp.splits[1];
+    const int64_t pairs = ((int64_t)rows * R.parts + 2 * R.tokens - 1) / (2 * R.tokens) + std::min(C.seqs, rows);
+    const int64_t items = pairs * C.kv_heads * P.sp.splits[1];
     if (items > 0x3fffffff) return "too many rows";
     CUtensorMap mq, mk, mv;
     if (!query_map(&mq, kv, q, q_ld, heads, rows) || !pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v))
@@ -336,17 +336,19 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
            qt, q_ld, heads, cu_q, kv_len, rows, scale * 1.44269504f, P.sp.per[0], P.sp.splits[0], P.chunk ? 1 : 0, ot, out_ld,
            part);
   }
-  if ((P.sp.splits[0] > 1 && !P.join) || P.sp.splits[1] > 1) {
+  const bool small = P.sp.splits[0] > 1 && !P.join, large = P.sp.splits[1] > 1;  // whose splits are left
+  if (small || large) {
     // a group of threads for every kCombineRun splits, as far as a block goes
-    const int most = std::max(P.join ? 1 : P.sp.splits[0], P.sp.splits[1]);
+    const int most = std::max(small ? P.sp.splits[0] : 1, P.sp.splits[1]);
     int groups_log2 = 0;
     while (most > kCombineRun << groups_log2 && D / 8 << groups_log2 < kCombineThreads) ++groups_log2;
-    const int64_t grid = (((int64_t)rows * heads * (D / 8) << groups_log2) + kCombineThreads - 1) / kCombineThreads;
-    if (grid > 0x7fffffff) return "too many rows";
-    SplitPlan sp = P.sp;
-    if (P.join) sp.splits[0] = 1;  // those have been joined
-    launch(true, k_paged_combine<O, D>, (unsigned)grid, kCombineThreads, 0, st, 1, C, heads, cu_q, kv_len, rows, sp,
-           groups_log2, part, ot, out_ld);
+    const int tile_rows = (int)std::min<int64_t>(kDecodeRows, (int64_t)std::max(max_q, 1) * (heads / C.kv_heads));
+    auto blocks = [&](int64_t units) { return ((units * (D / 8) << groups_log2) + kCombineThreads - 1) / kCombineThreads; };
+    const int64_t b0 = small ? blocks((int64_t)C.seqs * C.kv_heads * tile_rows) : 0;
+    const int64_t b1 = large ? blocks((int64_t)rows * heads) : 0;
+    if (b0 + b1 > 0x7fffffff) return "too many rows";
+    launch(true, k_paged_combine<O, D>, (unsigned)(b0 + b1), kCombineThreads, 0, st, 1, C, heads, cu_q, kv_len, rows, P.sp,
+           (int)b0, tile_rows, groups_log2, part, ot, out_ld);
   }
   return nullptr;
 }
@@ -370,7 +372,7 @@ const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, i
     using T = decltype(c);
     using O = decltype(o);
     auto* fn = kv->head_dim == 64 ? attention<T, O, 64> : attention<T, O, 128>;
-    return fn(kv, P, C, dev, q, q_ld, heads, cu_q, kv_len, rows, scale, out, out_ld, static_cast<float*>(workspace), waits,
+    return fn(kv, P, C, dev, q, q_ld, heads, cu_q, kv_len, rows, max_q, scale, out, out_ld, static_cast<float*>(workspace), waits,
               st, chained);
   };
   auto by_type = [&](auto c) { return out_type == LLAMA_F32 ? run(c, 0.0f) : run(c, c); };
