@@ -516,3 +516,51 @@ def test_calls_on_a_side_stream_are_ordered(pkg, lib):
     s.synchronize()
     del keep
     check_attention(pool, q, 32, [1], [600], out)
+
+
+@pytest.mark.parametrize("news", [[1, 2], [90, 3]])
+@pytest.mark.parametrize("scale", [0.0, 1e-6, 0.6, -0.125])
+def test_attention_scales(pkg, lib, news, scale):
+    """A scale of zero is the mean of the keys' values, a negative one attends with -q."""
+    import torch
+    lens = [700, 150]
+    pool = Pool(pkg, torch.bfloat16, 2, 128, 32, lens, seed=31)
+    pool.fill(lens)
+    q = torch.randn((sum(news), 8 * 128), device="cuda").bfloat16()
+    out = torch.zeros_like(q)
+    attend(pkg, lib, pool, q, 8, news, lens, out, scale=scale)
+    check_attention(pool, -q if scale < 0 else q, 8, news, lens, out, scale=abs(scale))
+
+
+def test_calls_at_once(pkg, lib):
+    """Calls on several streams, each with its workspace, give the bits that they give alone."""
+    import torch
+    shapes = [(64, 32, 8, [1] * 20, [100 * i + 7 for i in range(20)]), (128, 28, 4, [200, 1, 330, 1], [900, 3000, 330, 40]),
+              (64, 8, 8, [1], [9000]), (128, 16, 2, [150], [1200])]
+    jobs, alone = [], []
+    for i, (d, heads, kvh, news, lens) in enumerate(shapes):
+        pool = Pool(pkg, torch.float16, kvh, d, 16, lens, seed=40 + i)
+        pool.fill(lens)
+        q = torch.randn((sum(news), heads * d), device="cuda").half()
+        out = torch.zeros_like(q)
+        attend(pkg, lib, pool, q, heads, news, lens, out)
+        check_attention(pool, q, heads, news, lens, out)
+        alone.append(out)
+        cu = torch.tensor(np.cumsum([0] + news), dtype=torch.int32, device="cuda")
+        kvl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        size = lib.llama_paged_attention_workspace(ctypes.byref(pool.desc), heads, len(q), max(news), max(lens))
+        ws = torch.empty((size + 16,), dtype=torch.uint8, device="cuda")
+        jobs.append((pool, q, heads, news, lens, cu, kvl, size, ws, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[torch.zeros_like(j[1]) for j in jobs] for _ in range(6)]
+    torch.cuda.synchronize()
+    for row in outs:
+        for (pool, q, heads, news, lens, cu, kvl, size, ws, s), out in zip(jobs, row):
+            rc = lib.llama_paged_attention(ctypes.byref(pool.desc), q.data_ptr(), q.stride(0), heads, cu.data_ptr(),
+                                           kvl.data_ptr(), len(q), max(news), max(lens), pool.d ** -0.5, out.data_ptr(),
+                                           pkg.F16, out.stride(0), ws.data_ptr(), size, s.cuda_stream)
+            assert rc == 0
+    torch.cuda.synchronize()
+    for row in outs:
+        for out, want in zip(row, alone):
+            assert torch.equal(out, want)
