@@ -188,3 +188,14 @@ def test_rows_do_not_depend_on_each_other(pkg, lib):
     replayed = out.clone()
     call(0, n)
     assert torch.equal(out, replayed)
+
+
+@pytest.mark.parametrize("rows,vocab", [(149, 3001), (321, 700), (1024, 257), (1025, 130), (40, 128256)])
+def test_many_rows_of_mixed_rules(pkg, lib, rows, vocab):
+    """More rows than run at once: every row is taken exactly once, whatever its rule."""
+    import torch
+    rng = np.random.default_rng(rows)
+    pick = lambda *v: [v[i] for i in rng.integers(0, len(v), rows)]  # noqa: E731
+    lg = rand(rows, vocab, torch.float32, seed=rows, scale=1.0)
+    run(pkg, lib, lg, t=pick(0.0, 0.7, 1.2), k=pick(0, 0, 40, 3000), p=pick(1.0, 0.9, 0.97, 0.5), m=pick(0.0, 0.02),
+        u=rng.random(rows))
