@@ -531,7 +531,12 @@ __global__ void __launch_bounds__(kThreads)
   Scale S;
   S.top = logit_of((uint32_t)(best >> 32));
   S.c = 1.4426950408889634074 / (double)temp;
-  S.least = (float)fmax((double)S.top - 50.0 / S.c, -3.0e38);
+  // rounded down, and below top whatever fp32's (or fp64's) spacing there.  Where a spacing is so many
+  // temperatures that least would leave the exponent's range, nothing lies between it and top: any
+  // smaller distance that rounds to no weight will do.
+  S.least = fminf(__double2float_rd(fmax((double)S.top - 50.0 / S.c, -3.0e38)), nextafterf(S.top, -INFINITY));
+  const double reach = (double)S.top - (double)S.least;
+  if (reach * S.c > 900.0) S.c = 900.0 / reach;
   S.wide = !(S.least > kMasked);
   // bins over somewhat more than the range of the threads' maxima, or over what has weight
   // (exp(-32) < 2^-44); what lies below shares the last bin

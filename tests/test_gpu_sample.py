@@ -199,3 +199,46 @@ def test_many_rows_of_mixed_rules(pkg, lib, rows, vocab):
     lg = rand(rows, vocab, torch.float32, seed=rows, scale=1.0)
     run(pkg, lib, lg, t=pick(0.0, 0.7, 1.2), k=pick(0, 0, 40, 3000), p=pick(1.0, 0.9, 0.97, 0.5), m=pick(0.0, 0.02),
         u=rng.random(rows))
+
+
+@pytest.mark.parametrize("vocab", [3001, 50257])
+@pytest.mark.parametrize("top", [2e9, 1e20, 3e38, -5e29])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_maxima_whose_spacing_exceeds_the_temperature(pkg, lib, dtype, top, vocab):
+    """Row maxima so large that fp32's next lower value is many temperatures away: only equals of the
+    maximum have weight, whatever the rules, and masked ids (and the slots behind the row) have none."""
+    import torch
+    dt = getattr(torch, dtype)
+    rng = np.random.default_rng(vocab)
+    n = 24
+    lg = rand(n, vocab, dt, seed=vocab) if top > 0 else torch.full((n, vocab), -9e29, device="cuda").to(dt)
+    lg[:, ::5] = -math.inf
+    lg[:, 1::7] = math.nan
+    lg[:, 2::9] = -2e30
+    lg[:, [vocab // 3, vocab // 3 + 1, vocab - 1]] = top
+    if dtype == "float32":
+        lg[::2, 8] = float(np.nextafter(np.float32(top), np.float32(-np.inf)))
+    u = np.linspace(0, 1 - 2.0 ** -24, n)
+    for t in (0.02, 0.7, 1.0):
+        run(pkg, lib, lg, t=t, u=u)
+        run(pkg, lib, lg, t=t, u=u, p=0.9)
+        run(pkg, lib, lg, t=t, u=u, k=rng.choice([0, 1, 2, 3, 40, 2500], n), p=rng.choice([1.0, 0.3, 0.7], n),
+            m=rng.choice([0.0, 0.5], n))
+
+
+@pytest.mark.parametrize("top", [2.0 ** 31, 3e38])
+def test_maxima_with_a_few_spacings_to_the_temperature(pkg, lib, top):
+    """The logits with weight lie within a few fp32 steps of the maximum; the many below them have none,
+    not even together (the last random number below 1 falls on the last id with weight)."""
+    import torch
+    vocab = 200001
+    step = float(np.float32(top)) - float(np.nextafter(np.float32(top), np.float32(-np.inf)))
+    for factor in (0.014, 0.03, 0.04, 0.06, 0.3, 2.0):
+        t = np.float32(step * factor)
+        lg = torch.zeros((6, vocab), device="cuda")
+        lg[:, 0] = top
+        near = torch.tensor([np.float32(top - step * i) for i in range(1, 40)], device="cuda")
+        lg[3:, 1:40] = near
+        lg[4, 100:] = -math.inf
+        for p in (1.0, 0.99999994, 0.5):
+            run(pkg, lib, lg, t=t, p=p, u=[1 - 2.0 ** -24, 0.5, 0.0, 1 - 2.0 ** -24, 1 - 2.0 ** -24, 0.9])
