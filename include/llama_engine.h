@@ -221,6 +221,10 @@ int llama_engine_decode_path(llama_engine_t engine);
  * 0 = token by token through the decode path.  -1 for a NULL handle. */
 int llama_engine_batch_path(llama_engine_t engine);
 
+/* Steps of the batched path that were launched as a captured CUDA graph so far (diagnostic; the
+ * others were launched kernel by kernel).  -1 for a NULL handle. */
+long long llama_engine_graph_steps(llama_engine_t engine);
+
 /* Diagnostics for the persistent kernel: enable = 1 starts recording a phase trace of the first
  * token of each following launch (globaltimer timestamps per CTA at every phase's start, after
  * its dependency wait, after staging and at its end), 0 stops, 2 copies up to max_entries

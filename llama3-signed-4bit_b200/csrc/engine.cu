@@ -12,6 +12,7 @@
 #include <unistd.h>
 
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <cstddef>
 #include <cmath>
@@ -244,10 +245,17 @@ struct Engine {
   int tc_expire = 0;                        // test hook: the GEMM's issuer waits on nothing
   int attn_expire = 0;                      // test hook: the prefill attention's issuer waits on nothing
   unsigned long long attn_wait_ns = kWaitNs;  // bound on the prefill attention's waits (test hook)
-  // decode steps of the batched path replayed as CUDA graphs, one per (rows, logits rows,
-  // attention splits); the rows' ids, positions and slots are read from t_idx
-  struct TcGraph { int n, nlog, splits; bool fold; int runs, run_q, run_kv; cudaGraphExec_t exec; };
+  // steps of the batched path replayed as CUDA graphs, one per shape (tc_step_graph's key); the rows'
+  // ids, positions and slots are read from t_idx.  Shapes that were seen are kept with and without one.
+  struct TcGraph {
+    std::array<int, 7> key;
+    cudaGraphExec_t exec;
+    int seen;        // steps since the shape was noted
+    long long last;  // step of its last use
+  };
   std::vector<TcGraph> tc_graphs;
+  long long tc_steps = 0;     // forward_batch and forward_token steps so far
+  long long graph_steps = 0;  // batched steps launched as a graph
   // token scoring (llama_engine_score_tokens): logits of a chunk's rows, targets, results
   float* sc_logits = nullptr;   // [kScoreRows][vocab], allocated on first use
   int32_t* sc_target = nullptr; // [kScoreRows]
@@ -1210,32 +1218,65 @@ static bool tc_step(Engine* E, int n, int lrow0, int nlog, int max_pos, int pref
   return true;
 }
 
-// A decode step (rows already uploaded) through a cached CUDA graph of tc_step's launches.
+// A step of any rows (already uploaded) through a cached CUDA graph of tc_step's launches.  A shape is what
+// the launches depend on: rows and logits rows, and of a flat engine the attention splits and fold, of a
+// paged one the runs and the bounds of their rows and keys.  It is captured when it is first seen;
+// a paged step with prompts in it when it is seen again, since prompts' lengths rarely are, and with
+// kGraphs held on its fourth step, in the place of the graph whose last use is the longest ago.  A
+// capture costs about as much as some steps launched kernel by kernel.
+constexpr size_t kGraphs = 64, kGraphShapes = 256;
 static bool tc_step_graph(Engine* E, int n, int nlog, int max_pos, bool fold) {
-  const int splits = attn_splits_for(max_pos);
-  for (const auto& g : E->tc_graphs)
-    if (g.n == n && g.nlog == nlog && g.splits == splits && g.fold == fold && g.runs == E->runs && g.run_q == E->run_q &&
-        g.run_kv == E->run_kv) {
-      LE_CK(cudaGraphLaunch(g.exec, E->stream));
-      E->tc_dirty = true;
-      return true;
-    }
-  if (E->tc_graphs.size() >= 64) return tc_step(E, n, 0, nlog, max_pos, -1, nullptr, fold);  // launch directly
-  LE_CK(cudaStreamBeginCapture(E->stream, cudaStreamCaptureModeThreadLocal));
-  const bool ok = tc_step(E, n, 0, nlog, max_pos, -1, nullptr, fold);
-  cudaGraph_t graph = nullptr;
-  const cudaError_t ce = cudaStreamEndCapture(E->stream, &graph);
-  if (!ok || ce != cudaSuccess || graph == nullptr) {
-    if (graph) cudaGraphDestroy(graph);
-    E->err = std::string("batched step capture failed: ") + cudaGetErrorString(ce);
-    return false;
+  const std::array<int, 7> key = {n,
+                                  nlog,
+                                  E->paged ? 0 : attn_splits_for(max_pos),
+                                  E->paged ? 0 : (int)fold,
+                                  E->runs,
+                                  E->run_q,
+                                  E->run_kv};
+  auto& all = E->tc_graphs;
+  auto oldest = [&](bool with) {  // the shape with (or without) a graph that was used the longest ago
+    size_t at = all.size();
+    for (size_t i = 0; i < all.size(); ++i)
+      if ((all[i].exec != nullptr) == with && (at == all.size() || all[i].last < all[at].last)) at = i;
+    return at;
+  };
+  size_t at = 0;
+  while (at < all.size() && all[at].key != key) ++at;
+  if (at == all.size()) {
+    if (all.size() >= kGraphShapes) at = oldest(false);
+    else all.emplace_back();
+    all[at] = {key, nullptr, 0, 0};
   }
-  cudaGraphExec_t exec = nullptr;
-  const cudaError_t ie = cudaGraphInstantiate(&exec, graph, 0);
-  cudaGraphDestroy(graph);
-  if (ie != cudaSuccess) { E->err = cudaGetErrorString(ie); return false; }
-  E->tc_graphs.push_back({n, nlog, splits, fold, E->runs, E->run_q, E->run_kv, exec});
-  LE_CK(cudaGraphLaunch(exec, E->stream));
+  all[at].last = ++E->tc_steps;
+  if (!all[at].exec) {
+    size_t held = 0;
+    for (const auto& g : all) held += g.exec ? 1 : 0;
+    const int wanted = held >= kGraphs ? 4 : E->paged && E->runs < n ? 2 : 1;
+    if (++all[at].seen < wanted) return tc_step(E, n, 0, nlog, max_pos, -1, nullptr, fold);
+    LE_CK(cudaStreamBeginCapture(E->stream, cudaStreamCaptureModeThreadLocal));
+    const bool ok = tc_step(E, n, 0, nlog, max_pos, -1, nullptr, fold);
+    cudaGraph_t graph = nullptr;
+    const cudaError_t ce = cudaStreamEndCapture(E->stream, &graph);
+    if (!ok || ce != cudaSuccess || graph == nullptr) {
+      if (graph) cudaGraphDestroy(graph);
+      E->err = std::string("batched step capture failed: ") + cudaGetErrorString(ce);
+      return false;
+    }
+    cudaGraphExec_t exec = nullptr;
+    const cudaError_t ie = cudaGraphInstantiate(&exec, graph, 0);
+    cudaGraphDestroy(graph);
+    if (ie != cudaSuccess) { E->err = cudaGetErrorString(ie); return false; }
+    if (held >= kGraphs) {  // its running launches end before it is freed
+      auto& old = all[oldest(true)];
+      cudaGraphExecDestroy(old.exec);
+      old.exec = nullptr;
+      old.seen = 0;
+    }
+    all[at].exec = exec;
+  }
+  LE_CK(cudaGraphLaunch(all[at].exec, E->stream));
+  E->tc_dirty = true;
+  ++E->graph_steps;
   return true;
 }
 
@@ -2320,6 +2361,8 @@ LE_API int llama_engine_batch_path(llama_engine_t engine) {
   if (!engine) return -1;
   return H(engine)->tc ? 1 : 0;
 }
+
+LE_API long long llama_engine_graph_steps(llama_engine_t engine) { return engine ? H(engine)->graph_steps : -1; }
 
 LE_API void* llama_engine_get_stream(llama_engine_t engine) { return engine ? (void*)H(engine)->stream : nullptr; }
 

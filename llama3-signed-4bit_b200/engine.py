@@ -85,6 +85,8 @@ class LlamaEngineBindings:
         lib.llama_engine_decode_path.restype = ctypes.c_int
         lib.llama_engine_batch_path.argtypes = [_P]
         lib.llama_engine_batch_path.restype = ctypes.c_int
+        lib.llama_engine_graph_steps.argtypes = [_P]
+        lib.llama_engine_graph_steps.restype = ctypes.c_longlong
         lib.llama_engine_trace.argtypes = [_P, ctypes.c_int, ctypes.c_void_p, ctypes.c_int]
         lib.llama_engine_trace.restype = ctypes.c_int
         lib.llama_engine_get_stream.argtypes = [_P]
@@ -348,6 +350,11 @@ class LlamaEngine:
     def batch_path(self) -> str:
         """Implementation of prefill and forward_batch: "tensor-core" or "token-loop"."""
         return {1: "tensor-core", 0: "token-loop"}.get(self.bindings.lib.llama_engine_batch_path(self.handle), "?")
+
+    @property
+    def graph_steps(self) -> int:
+        """Batched steps that were launched as a captured CUDA graph so far."""
+        return self.bindings.lib.llama_engine_graph_steps(self.handle)
 
     def close(self):
         if getattr(self, "handle", None):

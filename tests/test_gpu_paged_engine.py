@@ -231,3 +231,56 @@ def test_create_refusals(pkg, bindings, small_model, chain_model):
     # a geometry without the tensor-core batched path
     assert not lib.llama_engine_create_paged(str(chain_model).encode(), 0, 1, 64, 4, 16, 1)
     assert b"batched path" in lib.llama_engine_last_error(None)
+
+
+def test_steps_are_captured_after_many_prompt_shapes(pkg, bindings, small_model):
+    """Prompts of ever new lengths take no decode step's graph: a decode shape that comes after them is
+    replayed from its first step on, a prompt's shape from its second.  Replays give the same bits."""
+    eng = pkg.LlamaEngine(str(small_model), bindings, device=0, max_batch=2, max_seq_len=128, num_pages=16, page_size=16)
+    try:
+        before = eng.graph_steps
+        for n in range(2, 82):
+            eng.forward_batch(list(range(n)), list(range(n)), [0] * n, compute_logits=False)
+            eng.release_slot(0)
+        assert eng.graph_steps == before
+        eng.prefill(list(range(20)), 0, False)
+        seen = []
+        for i in range(3):  # the same decode step again and again
+            eng.forward_batch([7, 9], [20, 0], [0, 1])
+            assert eng.graph_steps == before + i + 1
+            seen.append(np.stack([eng.get_logits_batch(r) for r in range(2)]))
+        assert all(np.array_equal(seen[0], x) for x in seen[1:])
+        before = eng.graph_steps
+        seen = []
+        for i in range(3):  # a prompt with a single token beside it: launched, then captured, then replayed
+            eng.forward_batch([7, 9, 11], [20, 0, 1], [0, 1, 1], compute_logits=False)
+            eng.forward_batch([7, 9], [21, 2], [0, 1])
+            assert eng.graph_steps == before + i + (i + 1)
+            seen.append(np.stack([eng.get_logits_batch(r) for r in range(2)]))
+        assert all(np.array_equal(seen[0], x) for x in seen[1:])
+    finally:
+        eng.close()
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_more_step_shapes_than_graphs(pkg, bindings, small_model, paged):
+    """A shape beyond the graphs that are held takes the place of the one used the longest ago once it has
+    come four times; results do not depend on which steps are replayed."""
+    extra = dict(num_pages=70, page_size=16) if paged else {}
+    eng = pkg.LlamaEngine(str(small_model), bindings, device=0, max_batch=70, max_seq_len=16, **extra)
+    try:
+        def step(n):
+            g = eng.graph_steps
+            eng.forward_batch(list(range(n)), [0] * n, list(range(n)))
+            return eng.graph_steps - g, eng.get_logits_batch(n - 1)
+
+        first = [step(n) for n in range(1, 71)]
+        assert [f[0] for f in first] == [1] * 64 + [0] * 6
+        for want in (0, 0, 1, 1):  # the last shape's second to fifth steps
+            got, logits = step(70)
+            assert got == want and np.array_equal(logits, first[69][1])
+        assert step(64)[0] == 1 and step(2)[0] == 1  # still held
+        got, logits = step(1)  # gave its place
+        assert got == 0 and np.array_equal(logits, first[0][1])
+    finally:
+        eng.close()
