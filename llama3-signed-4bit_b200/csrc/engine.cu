@@ -303,7 +303,7 @@ static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
   do {                                                                       \
     cudaError_t e_ = (expr);                                                 \
     if (e_ != cudaSuccess) {                                                 \
-      E->err = std::string(#expr) + ": " + cudaGetErrorString(e_);           \
+      E->err = std::string(#expr) + ": " + error_text(e_);                   \
       return false;                                                          \
     }                                                                        \
   } while (0)
@@ -2427,8 +2427,8 @@ LE_API int llama_engine_sample_batch(llama_engine_t engine, const float* tempera
   if (E->tp_world > 1) { E->err = "sample_batch: not available on a tensor-parallel engine"; return -1; }
   DeviceGuard dg(E->device);
   const size_t row = (size_t)E->max_batch;
-  if ((!E->d_sample && cudaMalloc(&E->d_sample, 6 * row * 4) != cudaSuccess) ||
-      (!E->h_sample && cudaMallocHost(&E->h_sample, 6 * row * 4) != cudaSuccess)) {
+  if ((!E->d_sample && error_text(cudaMalloc(&E->d_sample, 6 * row * 4))) ||
+      (!E->h_sample && error_text(cudaMallocHost(&E->h_sample, 6 * row * 4)))) {
     E->err = "sample_batch: out of memory";
     return -1;
   }
@@ -2438,14 +2438,14 @@ LE_API int llama_engine_sample_batch(llama_engine_t engine, const float* tempera
   for (int i = 0; i < 5; ++i)
     if (src[i]) std::memcpy(E->h_sample + i * row, src[i], (size_t)n * 4);
   auto dev = [&](int i) { return src[i] ? static_cast<void*>(E->d_sample + i * row) : nullptr; };
-  cudaError_t e = cudaMemcpyAsync(E->d_sample, E->h_sample, 5 * row * 4, cudaMemcpyHostToDevice, E->stream);
-  if (e == cudaSuccess)
-    e = sampling::sample_rows(E->logits, LLAMA_F32, E->vocab, n, (int)E->vocab, static_cast<float*>(dev(0)),
+  const char* why = error_text(cudaMemcpyAsync(E->d_sample, E->h_sample, 5 * row * 4, cudaMemcpyHostToDevice, E->stream));
+  if (!why)
+    why = sampling::sample_rows(E->logits, LLAMA_F32, E->vocab, n, (int)E->vocab, static_cast<float*>(dev(0)),
                               static_cast<int32_t*>(dev(1)), static_cast<float*>(dev(2)), static_cast<float*>(dev(3)),
                               static_cast<float*>(dev(4)), E->d_sample + 5 * row, E->device, E->stream);
-  if (e == cudaSuccess)
-    e = cudaMemcpyAsync(E->h_sample + 5 * row, E->d_sample + 5 * row, (size_t)n * 4, cudaMemcpyDeviceToHost, E->stream);
-  if (e != cudaSuccess) { E->err = std::string("sample_batch: ") + cudaGetErrorString(e); return -1; }
+  if (!why)
+    why = error_text(cudaMemcpyAsync(E->h_sample + 5 * row, E->d_sample + 5 * row, (size_t)n * 4, cudaMemcpyDeviceToHost, E->stream));
+  if (why) { E->err = std::string("sample_batch: ") + why; return -1; }
   if (!sync_ok(E)) return -1;  // reports a device error of the step
   std::memcpy(out_tokens, E->h_sample + 5 * row, (size_t)n * 4);
   return 0;

@@ -41,6 +41,14 @@ inline int device_of(const void* p) {
   return a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged ? a.device : -1;
 }
 
+// Text of a call's result, or nullptr for success.  The runtime also keeps a failed call's error as
+// its last one, where a later check would take it for its own: it is taken out.
+inline const char* error_text(cudaError_t e) {
+  if (e == cudaSuccess) return nullptr;
+  cudaGetLastError();
+  return cudaGetErrorString(e);
+}
+
 // Dynamic shared memory above 48 KB, allowed once per kernel and device.
 template <typename F>
 inline bool allow_smem(F* fn, int bytes, int dev) {
@@ -48,7 +56,7 @@ inline bool allow_smem(F* fn, int bytes, int dev) {
   static std::map<std::pair<const void*, int>, bool> done;
   std::lock_guard<std::mutex> lk(mu);
   bool& d = done[{reinterpret_cast<const void*>(fn), dev}];
-  if (!d) d = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  if (!d) d = !error_text(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   return d;
 }
 
@@ -76,9 +84,9 @@ const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, i
                            bool chained);
 }  // namespace paged
 
-// llama_sample_rows for checked arguments (sample_ops.cu).
+// llama_sample_rows for checked arguments (sample_ops.cu); nullptr, or why it failed.
 namespace sampling {
-cudaError_t sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
+const char* sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
                         const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
                         int32_t* out_ids, int dev, cudaStream_t st);
 }  // namespace sampling

@@ -133,9 +133,9 @@ static Cache cache_of(const llama_paged_kv_t* kv) {
 }
 
 // A launch that may start while the kernel before it runs out; that kernel's results are there
-// after its griddepcontrol.wait.
+// after its griddepcontrol.wait.  nullptr, or why it failed (an earlier call's error is not looked at).
 template <typename... KArgs, typename... Args>
-static void launch(bool early, void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
+static const char* launch(bool early, void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
                    int cluster, Args... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
@@ -154,7 +154,7 @@ static void launch(bool early, void (*kernel)(KArgs...), unsigned grid, unsigned
     at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  return error_text(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
 }
 
 const char* append_rows(const llama_paged_kv_t* kv, const void* qkv, int type, int64_t ld, int planes,
@@ -171,18 +171,13 @@ const char* append_rows(const llama_paged_kv_t* kv, const void* qkv, int type, i
     using Kv = decltype(c);
     using Q = decltype(q);
     auto* fn = D == 64 ? k_paged_append<In, Kv, Q, 64> : k_paged_append<In, Kv, Q, 128>;
-    launch(chained, fn, grid, 256, 0, st, 1, C, static_cast<const In*>(qkv), ld, planes, plane_stride, rows, heads, pos, seq,
-           rope_cos, rope_sin, n_pos, static_cast<Q*>(q_out), q_ld);
+    return launch(chained, fn, grid, 256, 0, st, 1, C, static_cast<const In*>(qkv), ld, planes, plane_stride, rows, heads, pos,
+                  seq, rope_cos, rope_sin, n_pos, static_cast<Q*>(q_out), q_ld);
   };
   auto by_type = [&](auto c) {
-    if (type != LLAMA_F32) run(c, c, c);
-    else if (q_type == LLAMA_F32) run(0.0f, c, 0.0f);
-    else run(0.0f, c, c);
+    return type != LLAMA_F32 ? run(c, c, c) : q_type == LLAMA_F32 ? run(0.0f, c, 0.0f) : run(0.0f, c, c);
   };
-  if (kv->type == LLAMA_F16) by_type(__half{});
-  else by_type(__nv_bfloat16{});
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+  return kv->type == LLAMA_F16 ? by_type(__half{}) : by_type(__nv_bfloat16{});
 }
 
 constexpr int kSms = 148;  // the workspace's size must not need a device
@@ -323,18 +318,20 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
     if (!query_map(&mq, kv, q, q_ld, heads, rows) || !pool_map(&mk, kv, kv->k) || !pool_map(&mv, kv, kv->v))
       return "tensor maps could not be made";
     if (!allow_smem(k_paged_chunk<T, O, D>, ChunkGeo<D>::kSmem, dev)) return "shared memory could not be set";
-    launch(chained, k_paged_chunk<T, O, D>, (unsigned)items, kChunkThreads, ChunkGeo<D>::kSmem, st, 1,
-           mq, mk, mv, C, heads, cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1], P.sp.splits[1], P.longest ? 1 : 0, ot, out_ld,
-           part + P.sp.part1 * (D + 8), waits);
+    if (const char* why = launch(chained, k_paged_chunk<T, O, D>, (unsigned)items, kChunkThreads, ChunkGeo<D>::kSmem, st, 1,
+                                 mq, mk, mv, C, heads, cu_q, kv_len, rows, scale, P.sp.small_rows, P.sp.per[1],
+                                 P.sp.splits[1], P.longest ? 1 : 0, ot, out_ld, part + P.sp.part1 * (D + 8), waits))
+      return why;
   }
   if (P.decode) {
     const int64_t grid = (int64_t)C.seqs * C.kv_heads * P.sp.splits[0];
     if (grid > 0x7fffffff) return "too many sequences";
     auto* fn = P.join ? k_paged_decode<T, O, D, true> : k_paged_decode<T, O, D, false>;
     if (!allow_smem(fn, DecodeGeo<D>::kSmem, dev)) return "shared memory could not be set";
-    launch(P.chunk || chained, fn, (unsigned)grid, 32 * kDecodeWarps, DecodeGeo<D>::kSmem, st, P.join ? P.sp.splits[0] : 1, C,
-           qt, q_ld, heads, cu_q, kv_len, rows, scale * 1.44269504f, P.sp.per[0], P.sp.splits[0], P.chunk ? 1 : 0, ot, out_ld,
-           part);
+    if (const char* why = launch(P.chunk || chained, fn, (unsigned)grid, 32 * kDecodeWarps, DecodeGeo<D>::kSmem, st,
+                                 P.join ? P.sp.splits[0] : 1, C, qt, q_ld, heads, cu_q, kv_len, rows, scale * 1.44269504f,
+                                 P.sp.per[0], P.sp.splits[0], P.chunk ? 1 : 0, ot, out_ld, part))
+      return why;
   }
   const bool small = P.sp.splits[0] > 1 && !P.join, large = P.sp.splits[1] > 1;  // whose splits are left
   if (small || large) {
@@ -347,8 +344,9 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
     const int64_t b0 = small ? blocks((int64_t)C.seqs * C.kv_heads * tile_rows) : 0;
     const int64_t b1 = large ? blocks((int64_t)rows * heads) : 0;
     if (b0 + b1 > 0x7fffffff) return "too many rows";
-    launch(true, k_paged_combine<O, D>, (unsigned)(b0 + b1), kCombineThreads, 0, st, 1, C, heads, cu_q, kv_len, rows, P.sp,
-           (int)b0, tile_rows, groups_log2, part, ot, out_ld);
+    if (const char* why = launch(true, k_paged_combine<O, D>, (unsigned)(b0 + b1), kCombineThreads, 0, st, 1, C, heads, cu_q,
+                                 kv_len, rows, P.sp, (int)b0, tile_rows, groups_log2, part, ot, out_ld))
+      return why;
   }
   return nullptr;
 }
@@ -376,9 +374,7 @@ const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, i
               st, chained);
   };
   auto by_type = [&](auto c) { return out_type == LLAMA_F32 ? run(c, 0.0f) : run(c, c); };
-  if (const char* why = kv->type == LLAMA_F16 ? by_type(__half{}) : by_type(__nv_bfloat16{})) return why;
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+  return kv->type == LLAMA_F16 ? by_type(__half{}) : by_type(__nv_bfloat16{});
 }
 
 }  // namespace paged

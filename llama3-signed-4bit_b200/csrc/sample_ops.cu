@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-cudaError_t sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
+const char* sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
                         const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
                         int32_t* out_ids, int dev, cudaStream_t st) {
   // CTAs of a row: as few as can hold it (up to 128 KB each: one CTA per SM), and more while that
@@ -690,14 +690,14 @@ cudaError_t sample_rows(const void* logits, int type, int64_t ld, int rows, int 
   const int64_t bytes = (int64_t)vocab * (type == LLAMA_F32 ? 4 : 2);
   int ranks = 1;
   while (ranks < kMaxCluster && (bytes > 131000 * (int64_t)ranks || rows * ranks < 148)) ranks *= 2;
-  auto launch = [&](auto x, auto r) {
+  auto launch = [&](auto x, auto r) -> const char* {
     using T = decltype(x);
     constexpr int R = decltype(r)::value;
     const int seg = (vocab + R - 1) / R;
     // a part and the slots before it, in whole groups for every warp
     const int groups = (int)(((int64_t)(seg + Part<T>::kRun) * sizeof(T) + 512 * kWarps - 1) / (512 * kWarps));
     const int smem = kSharedBytes + groups * kWarps * 512;
-    if (!allow_smem(k_sample_rows<R, T>, 224 * 1024, dev)) return cudaErrorInvalidValue;
+    if (!allow_smem(k_sample_rows<R, T>, 224 * 1024, dev)) return "shared memory could not be set";
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * R));
     cfg.blockDim = dim3(kThreads);
@@ -709,8 +709,8 @@ cudaError_t sample_rows(const void* logits, int type, int64_t ld, int rows, int 
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_sample_rows<R, T>, static_cast<const T*>(logits), ld, vocab, seg, groups,
-                              temperature, top_k, top_p, min_p, uniform, out_ids);
+    return error_text(cudaLaunchKernelEx(&cfg, k_sample_rows<R, T>, static_cast<const T*>(logits), ld, vocab, seg, groups,
+                                         temperature, top_k, top_p, min_p, uniform, out_ids));
   };
   auto by_ranks = [&](auto x) {
     switch (ranks) {
@@ -720,8 +720,7 @@ cudaError_t sample_rows(const void* logits, int type, int64_t ld, int rows, int 
       default: return launch(x, std::integral_constant<int, 8>{});
     }
   };
-  const cudaError_t e = type == LLAMA_F32 ? by_ranks(0.0f) : type == LLAMA_F16 ? by_ranks(__half{}) : by_ranks(__nv_bfloat16{});
-  return e == cudaSuccess ? cudaGetLastError() : e;
+  return type == LLAMA_F32 ? by_ranks(0.0f) : type == LLAMA_F16 ? by_ranks(__half{}) : by_ranks(__nv_bfloat16{});
 }
 
 static int refuse(const char* why, int rc = -1) {
@@ -751,7 +750,7 @@ LE_API int llama_sample_rows(const void* logits, int type, int64_t ld, int rows,
   for (const void* p : ptrs)
     if (p && device_of(p) != dev) return refuse("every pointer must be memory of one CUDA device");
   DeviceGuard dg(dev);
-  const cudaError_t e = sample_rows(logits, type, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out_ids, dev,
-                                    static_cast<cudaStream_t>(stream));
-  return e == cudaSuccess ? 0 : refuse(cudaGetErrorString(e));
+  const char* why = sample_rows(logits, type, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out_ids, dev,
+                                static_cast<cudaStream_t>(stream));
+  return why ? refuse(why) : 0;
 }

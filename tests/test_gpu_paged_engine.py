@@ -284,3 +284,24 @@ def test_more_step_shapes_than_graphs(pkg, bindings, small_model, paged):
         assert got == 0 and np.array_equal(logits, first[0][1])
     finally:
         eng.close()
+
+
+def test_operators_after_a_create_that_ran_out_of_memory(pkg, bindings, small_model):
+    """An engine that could not be made leaves nothing behind that a later call would report as its own."""
+    import torch
+    lib = bindings.lib
+    lg = torch.randn((3, 1000), device="cuda")
+    u = torch.rand(3, device="cuda")
+    ids = torch.full((3,), -5, dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        assert not lib.llama_engine_create_paged(str(small_model).encode(), 0, 1, 64, 2 ** 31 - 1, 256, 1)
+        assert b"out of memory" in lib.llama_engine_last_error(None)
+        assert lib.llama_sample_rows(lg.data_ptr(), pkg.F32, 1000, 3, 1000, None, None, None, None, u.data_ptr(),
+                                     ids.data_ptr(), 0) == 0, lib.llama_engine_last_error(None)
+    assert not lib.llama_engine_create_paged(str(small_model).encode(), 0, 1, 64, 2 ** 31 - 1, 256, 1)
+    eng = pkg.LlamaEngine(str(small_model), bindings, device=0, max_batch=1, max_seq_len=64, num_pages=4, page_size=16)
+    try:
+        eng.forward_token(5, 0, True)
+        assert eng.sample_batch([0.5], temperature=0.0) == [int(np.argmax(eng.get_logits_batch(0)))]
+    finally:
+        eng.close()
