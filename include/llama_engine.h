@@ -290,7 +290,8 @@ int llama_engine_check_schedule(int layers, int dim, int ffn_dim, int vocab_size
  * writes, so that the wait runs out: the persistent kernel's CTA 0 at the start of a launch, the
  * GEMM's MMA issuer before its first block; expire_code = 20 instead expires only the prefill
  * attention kernel (its MMA-issuing thread, after the first K / V tile copies are in flight),
- * and the GEMMs then keep the default bound, so that only the attention's wait runs out.  The launch
+ * and the GEMMs then keep the default bound, so that only the attention's wait runs out;
+ * expire_code = 21 expires only the row sampler of llama_engine_sample_batch.  The launch
  * then drains and the next waiting call fails with the timeout reported; expire_code = 0 turns
  * that off again and clears the recorded error so the engine can be used again.  Returns 0, or
  * -1 for a NULL handle. */

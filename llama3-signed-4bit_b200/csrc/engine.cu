@@ -147,6 +147,7 @@ static bool tc_pair_enabled() {
   return on;
 }
 constexpr int kExpireAttn = 20;  // llama_engine_debug_waits code that expires only the prefill attention
+constexpr int kExpireSample = 21;  // only the row sampler
 constexpr int kAttnMaxSplits = 8;
 constexpr int kScoreRows = 256;  // rows of logits held at once by llama_engine_score_tokens
 
@@ -275,6 +276,7 @@ struct Engine {
   // batched sampling (llama_engine_sample_batch): 5 parameters and the id of each row
   int32_t* d_sample = nullptr;   // [6][max_batch]
   int32_t* h_sample = nullptr;
+  sampling::Waits sample_waits;  // bound on the sampler's wait (test hook)
 
   cudaGraphExec_t g_fwd[2] = {nullptr, nullptr};  // [compute_logits]
   cudaGraphExec_t g_gen = nullptr;                // forward + greedy + advance
@@ -2309,14 +2311,17 @@ LE_API int llama_engine_debug_waits(llama_engine_t engine, unsigned long long wa
   if (cudaStreamSynchronize(E->stream) != cudaSuccess) return -1;
   const unsigned long long ns = wait_ns ? wait_ns : kWaitNs;
   E->pargs.wait_ns = ns;
-  E->pargs.expire_where = expire_code;
+  E->pargs.expire_where = expire_code == kExpireSample ? 0 : expire_code;
   // expiring only the attention keeps the default bound on the GEMMs: with programmatic launches
   // the next GEMM may already wait for the stalled attention's output, and its bounded waits
   // would otherwise run out in the same millisecond and race the attention's error code
-  E->tc_wait_ns = expire_code == kExpireAttn ? kWaitNs : ns;
+  E->tc_wait_ns = expire_code == kExpireAttn || expire_code == kExpireSample ? kWaitNs : ns;
   E->attn_wait_ns = ns;
-  E->tc_expire = expire_code != 0 && expire_code != kExpireAttn ? 1 : 0;
+  E->tc_expire = expire_code != 0 && expire_code != kExpireAttn && expire_code != kExpireSample ? 1 : 0;
   E->attn_expire = expire_code == kExpireAttn ? 1 : 0;
+  E->sample_waits = sampling::Waits();
+  if (wait_ns) E->sample_waits.ns = wait_ns;
+  E->sample_waits.expire = expire_code == kExpireSample ? 1 : 0;
   // captured batched steps hold the old GEMM arguments
   for (auto& g : E->tc_graphs)
     if (g.exec) cudaGraphExecDestroy(g.exec);
@@ -2442,12 +2447,14 @@ LE_API int llama_engine_sample_batch(llama_engine_t engine, const float* tempera
   if (!why)
     why = sampling::sample_rows(E->logits, LLAMA_F32, E->vocab, n, (int)E->vocab, static_cast<float*>(dev(0)),
                               static_cast<int32_t*>(dev(1)), static_cast<float*>(dev(2)), static_cast<float*>(dev(3)),
-                              static_cast<float*>(dev(4)), E->d_sample + 5 * row, E->device, E->stream);
+                              static_cast<float*>(dev(4)), E->d_sample + 5 * row, E->sample_waits, E->device, E->stream);
   if (!why)
     why = error_text(cudaMemcpyAsync(E->h_sample + 5 * row, E->d_sample + 5 * row, (size_t)n * 4, cudaMemcpyDeviceToHost, E->stream));
   if (why) { E->err = std::string("sample_batch: ") + why; return -1; }
   if (!sync_ok(E)) return -1;  // reports a device error of the step
-  std::memcpy(out_tokens, E->h_sample + 5 * row, (size_t)n * 4);
+  const int32_t* ids = E->h_sample + 5 * row;
+  if (*std::min_element(ids, ids + n) < 0) { E->err = "sample_batch: a row's copy timed out"; return -1; }
+  std::memcpy(out_tokens, ids, (size_t)n * 4);
   return 0;
 }
 

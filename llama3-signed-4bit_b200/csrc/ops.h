@@ -86,9 +86,14 @@ const char* attention_rows(const llama_paged_kv_t* kv, int dev, const void* q, i
 
 // llama_sample_rows for checked arguments (sample_ops.cu); nullptr, or why it failed.
 namespace sampling {
+// The bound on the wait for a row's copy, and (test only) whether it waits on what nothing completes.
+struct Waits {
+  unsigned long long ns = 4000000000ull;
+  int expire = 0;
+};
 const char* sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
                         const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
-                        int32_t* out_ids, int dev, cudaStream_t st);
+                        int32_t* out_ids, const Waits& waits, int dev, cudaStream_t st);
 }  // namespace sampling
 
 }  // namespace le

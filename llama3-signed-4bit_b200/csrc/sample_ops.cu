@@ -428,11 +428,11 @@ __global__ void __launch_bounds__(kThreads)
     k_sample_rows(const T* __restrict__ logits, int64_t ld, int vocab, int seg, int groups,
                   const float* __restrict__ temperature, const int32_t* __restrict__ top_k,
                   const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniform,
-                  int32_t* __restrict__ out) {
+                  int32_t* __restrict__ out, Waits W) {
   extern __shared__ __align__(16) uint8_t s_dyn[];
   Shared& sh = *reinterpret_cast<Shared*>(s_dyn);
   uint8_t* const s_part = s_dyn + kSharedBytes;
-  __shared__ __align__(8) u64 s_bar;
+  __shared__ __align__(8) u64 s_bar, s_never;  // the copy's, and (test only) one that nothing completes
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), row = blockIdx.x / R, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   cl.barrier_arrive();  // waited for before the first access to another CTA's memory
@@ -446,6 +446,7 @@ __global__ void __launch_bounds__(kThreads)
   T* slots = reinterpret_cast<T*>(s_part);
   if (tid == 0) {
     mbar_init(smem_u32(&s_bar), 1);
+    mbar_init(smem_u32(&s_never), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     mbar_expect_tx(smem_u32(&s_bar), (uint32_t)body * sizeof(T));
     if (body) bulk_g2s(smem_u32(slots + off + head), src + head, (uint32_t)body * sizeof(T), smem_u32(&s_bar));
@@ -463,11 +464,14 @@ __global__ void __launch_bounds__(kThreads)
   const float p = top_p ? top_p[row] : 1.0f, mp = min_p ? min_p[row] : 0.0f, u = uniform[row];
   if (tid < kTable) sh.table[tid] = exp2((double)tid / kTable);
   __syncthreads();
-  bool late = false;  // the copy did not come within the bound (4 s): the row's id becomes -1
-  {
+  auto wait = [&](u64* bar) {
     const unsigned long long t0 = gtimer();
-    while (!late && !mbar_try(smem_u32(&s_bar), 0)) late = gtimer() - t0 > 4000000000ull;
-  }
+    while (!mbar_try(smem_u32(bar), 0))
+      if (gtimer() - t0 > W.ns) return false;
+    return true;
+  };
+  bool late = !wait(W.expire ? &s_never : &s_bar);  // no copy within the bound: the row's id becomes -1
+  if (late) wait(&s_bar);  // once more: it shall not land where another CTA's memory is by then
   // maximum with its lowest index (of the unmasked), and the lowest of the threads' maxima
   float mine = kMasked;
   uint32_t at = 0;
@@ -684,7 +688,7 @@ __global__ void __launch_bounds__(kThreads)
 
 const char* sample_rows(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temperature,
                         const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
-                        int32_t* out_ids, int dev, cudaStream_t st) {
+                        int32_t* out_ids, const Waits& waits, int dev, cudaStream_t st) {
   // CTAs of a row: as few as can hold it (up to 128 KB each: one CTA per SM), and more while that
   // leaves SMs idle; measured at 256 x 50257 bf16 ids without truncation: 1 CTA a row 35 us, 4 CTAs 71 us
   const int64_t bytes = (int64_t)vocab * (type == LLAMA_F32 ? 4 : 2);
@@ -710,7 +714,7 @@ const char* sample_rows(const void* logits, int type, int64_t ld, int rows, int 
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return error_text(cudaLaunchKernelEx(&cfg, k_sample_rows<R, T>, static_cast<const T*>(logits), ld, vocab, seg, groups,
-                                         temperature, top_k, top_p, min_p, uniform, out_ids));
+                                         temperature, top_k, top_p, min_p, uniform, out_ids, waits));
   };
   auto by_ranks = [&](auto x) {
     switch (ranks) {
@@ -750,7 +754,7 @@ LE_API int llama_sample_rows(const void* logits, int type, int64_t ld, int rows,
   for (const void* p : ptrs)
     if (p && device_of(p) != dev) return refuse("every pointer must be memory of one CUDA device");
   DeviceGuard dg(dev);
-  const char* why = sample_rows(logits, type, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out_ids, dev,
-                                static_cast<cudaStream_t>(stream));
+  const char* why = sample_rows(logits, type, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out_ids, Waits(),
+                                dev, static_cast<cudaStream_t>(stream));
   return why ? refuse(why) : 0;
 }

@@ -305,3 +305,24 @@ def test_operators_after_a_create_that_ran_out_of_memory(pkg, bindings, small_mo
         assert eng.sample_batch([0.5], temperature=0.0) == [int(np.argmax(eng.get_logits_batch(0)))]
     finally:
         eng.close()
+
+
+def test_a_sampled_row_whose_wait_runs_out_is_reported(pkg, bindings, small_model):
+    """The sampler waits for a copy that never comes (1 ms bound): the call fails, no id is returned, and
+    the engine works again."""
+    eng = pkg.LlamaEngine(str(small_model), bindings, device=0, max_batch=3, max_seq_len=64)
+    lib = bindings.lib
+    try:
+        eng.forward_batch([5, 6, 7], [0, 0, 0], [0, 1, 2])
+        ref = eng.sample_batch([0.2, 0.5, 0.9], top_k=40)
+        assert lib.llama_engine_debug_waits(eng.handle, 1_000_000, 21) == 0
+        for rules in (dict(), dict(top_k=40), dict(top_p=0.9), dict(temperature=0.0)):
+            with pytest.raises(RuntimeError, match="timed out"):
+                eng.sample_batch([0.2, 0.5, 0.9], **rules)
+        eng.forward_batch([5, 6, 7], [0, 0, 0], [0, 1, 2])  # the step's own waits are not cut
+        with pytest.raises(RuntimeError, match="timed out"):
+            eng.sample_batch([0.2, 0.5, 0.9], top_k=40)
+        assert lib.llama_engine_debug_waits(eng.handle, 0, 0) == 0
+        assert eng.sample_batch([0.2, 0.5, 0.9], top_k=40) == ref
+    finally:
+        eng.close()
