@@ -65,8 +65,9 @@ inline bool allow_smem(F* fn, int bytes, int dev) {
 // its results themselves).
 namespace paged {
 constexpr uint32_t kChunkError = 30;  // error word of a wait of the chunk form that ran out
-// The chunk form's bounded waits: where it reports, the bound, and (test only) whether its product
-// issuer first waits on a barrier phase that nothing completes.
+// The chunk form's bounded waits: where it reports one that ran out (nullptr: the rows' NaN alone tell),
+// the bound, and (test only) whether its product issuer first waits on a barrier phase that nothing
+// completes.
 struct Waits {
   uint32_t* error = nullptr;
   unsigned long long ns = 2000000000ull;

@@ -33,7 +33,7 @@
 // Weights are rounded to the cache's type as the A operand of P V; their sum is taken in fp32 before
 // that.
 //
-// All mbarrier waits are bounded; on timeout the error word is set, every role stops, the copies and
+// All mbarrier waits are bounded; on timeout the engine's error word is set, every role stops, the copies and
 // products in flight are waited for (again bounded) and the rows of the items that the CTA had taken on
 // become NaN.
 //
@@ -152,7 +152,7 @@ __device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, volati
       if (t0 == 0) t0 = t;
       if (t - t0 > W.ns) {
         *abort = 1u;
-        atomicCAS(W.error, 0u, kChunkError);
+        if (W.error) atomicCAS(W.error, 0u, kChunkError);
         return false;
       }
     }

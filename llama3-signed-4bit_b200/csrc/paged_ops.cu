@@ -5,8 +5,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <map>
-#include <mutex>
 
 #include "common.cuh"
 #include "ops.h"
@@ -291,17 +289,6 @@ static bool query_map(CUtensorMap* m, const llama_paged_kv_t* kv, const void* q,
   return make_map(m, kv->type, 3, q, dims, strides, box);
 }
 
-// Device word that a wait which ran out in the chunk form sets (its rows become NaN as well).
-__device__ uint32_t g_paged_error;
-static uint32_t* error_word(int dev) {
-  static std::mutex mu;
-  static std::map<int, uint32_t*> at;
-  std::lock_guard<std::mutex> lk(mu);
-  uint32_t*& p = at[dev];
-  if (!p && cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_paged_error) != cudaSuccess) p = nullptr;
-  return p;
-}
-
 template <typename T, typename O, int D>
 static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Cache& C, int dev, const void* q, int64_t q_ld, int heads,
                              const int32_t* cu_q, const int32_t* kv_len, int rows, int max_q, float scale, void* out,
@@ -444,11 +431,8 @@ LE_API int llama_paged_attention(const llama_paged_kv_t* kv, const void* q, int6
   for (const void* p : ptrs)
     if (dev < 0 || (p && device_of(p) != dev)) return refuse(who, "every pointer must be memory of one CUDA device");
   DeviceGuard dg(dev);
-  Waits waits;
-  waits.error = error_word(dev);
-  if (!waits.error) return refuse(who, "the device's error word could not be found");
   if (const char* why = attention_rows(kv, dev, q, q_ld, heads, cu_q, kv_len, rows, max_q, max_kv, scale, out, out_type, out_ld,
-                                       workspace, waits, static_cast<cudaStream_t>(stream), false))
+                                       workspace, Waits(), static_cast<cudaStream_t>(stream), false))
     return refuse(who, why);
   return 0;
 }
