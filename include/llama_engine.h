@@ -370,8 +370,8 @@ int llama_paged_append(const llama_paged_kv_t* kv, const void* qkv, int type, in
  * sequence's new tokens (a sequence of more may be left unwritten) and max_kv a bound of kv_len that
  * only chooses how the work is split (any value is safe).  cu_q and kv_len are device memory, read
  * on the device: a captured call may be replayed over other lengths.  Keys and values of a
- * sequence's kv_len keys are finite; rows of its last page behind them may hold anything.  q and out are 16-byte
- * aligned and do not overlap, q_ld and out_ld multiples of 8.  workspace: 16-byte aligned device
+ * sequence's kv_len keys are finite (a row with a NaN score is NaN); rows of its last page behind them may
+ * hold anything.  q and out are 16-byte aligned and do not overlap, q_ld and out_ld multiples of 8.  workspace: 16-byte aligned device
  * memory of at least llama_paged_attention_workspace(...) bytes for the same arguments (NULL where that
  * is 0), whose contents need not be kept or cleared; calls that may overlap need one each.  Every
  * pointer is memory of one device; queued on `stream`.  Returns 0, -1 on bad arguments or a

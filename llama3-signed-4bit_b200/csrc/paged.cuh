@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kCombineThreads)
     }
   }
   if (used <= 1) return;
-  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  const float inv = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L;  // no key: zeros
 #pragma unroll
   for (int e = 0; e < 8; ++e) a[e] *= inv;
   store8(out + (int64_t)t * out_ld + (int64_t)h * D + d, a);

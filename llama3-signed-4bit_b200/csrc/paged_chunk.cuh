@@ -118,9 +118,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
 }
 
 constexpr uint32_t kNegInf = 0xff800000u;
+// Largest of three; NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // Two fp32 operations in one instruction.
@@ -702,10 +703,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             mx[x] = max3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
 #pragma unroll
             for (int e = 3; e < 15; e += 2) mx[x] = max3(mx[x], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-            mx[x] = fmaxf(mx[x], __uint_as_float(v[15]));
           }
+          mx[0] = max3(mx[0], __uint_as_float(u[0][15]), __uint_as_float(u[0][31]));
+          mx[1] = max3(mx[1], __uint_as_float(u[1][15]), __uint_as_float(u[1][31]));
           mt = max3(mt, max3(mx[0], mx[1], mx[2]), mx[3]);
         }
+        l = mt == mt ? l : mt;  // a score is NaN, so the row is: not all of the exponentials would pass it on
         // the product of the tile before: with P apart it may still read P and write O (in place, S was
         // computed behind it)
         if (Geo::kApart && tiles > 0) {

@@ -564,3 +564,27 @@ def test_calls_at_once(pkg, lib):
     for row in outs:
         for out, want in zip(row, alone):
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kvh,news,lens,bad", [
+    (2, [200], [500], [402, 440, 480]), (8, [1], [700], [650]), (2, [20], [9000], [8995]), (8, [1], [20000], [19000])])
+@pytest.mark.parametrize("kind,d", [("f16", 64), ("bf16", 128)])
+def test_attention_of_a_nan_key(pkg, lib, kind, d, kvh, news, lens, bad):
+    """A NaN among the keys that a row sees makes the row NaN, wherever the key lies in its tile (as the
+    formula has it); rows that do not see it are as without it."""
+    import torch
+    dt = types()[kind]
+    heads, n, kv = 4 * kvh, news[0], lens[0]
+    for first in range(bad[0], bad[0] + 8 if n == 200 else bad[0] + 4):
+        pool = Pool(pkg, dt, kvh, d, 16, lens, seed=50)
+        pool.fill(lens)
+        for j in [first] + bad[1:]:
+            pg, sl = pool.where(0, torch.tensor([j], device="cuda"))
+            pool.k[pg, sl, :, 3] = math.nan
+        q = torch.randn((n, heads * d), device="cuda").to(dt)
+        out = torch.zeros_like(q)
+        attend(pkg, lib, pool, q, heads, news, lens, out)
+        clear = max(0, first - (kv - n))  # rows whose position lies before the first bad key
+        assert bool(out[clear:].isnan().all()), (first, out[clear:].isnan().float().mean().item())
+        if clear:
+            check_attention(pool, q, heads, [clear], [kv - n + clear], out)
