@@ -658,7 +658,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   } else {
     // ---- softmax of row tile i, a thread per row ----
     const int i = warp >> 2;
-    const float c = fmaxf(fabsf(scale) * 1.44269504f, 1e-30f);  // > 0: a masked -inf stays -inf
+    // > 0, since a masked -inf has to stay -inf, but too small for any score where the scale is 0; and finite
+    const float c = fminf(fmaxf(fabsf(scale) * 1.44269504f, 1e-45f), 3.4e38f);
     const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const uint32_t t_s = lanes + 128u * i, t_p = lanes + Geo::kColP + Geo::kStepP * i, t_o = lanes + Geo::kColO + (uint32_t)(D * i);
     bool ok = true;

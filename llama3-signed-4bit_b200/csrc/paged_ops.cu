@@ -314,9 +314,10 @@ static const char* attention(const llama_paged_kv_t* kv, const Plan& P, const Ca
     const int64_t grid = (int64_t)C.seqs * C.kv_heads * P.sp.splits[0];
     if (grid > 0x7fffffff) return "too many sequences";
     auto* fn = P.join ? k_paged_decode<T, O, D, true> : k_paged_decode<T, O, D, false>;
+    const float scale_log2 = std::min(std::max(scale * 1.44269504f, -3.4e38f), 3.4e38f);
     if (!allow_smem(fn, DecodeGeo<D>::kSmem, dev)) return "shared memory could not be set";
     if (const char* why = launch(P.chunk || chained, fn, (unsigned)grid, 32 * kDecodeWarps, DecodeGeo<D>::kSmem, st,
-                                 P.join ? P.sp.splits[0] : 1, C, qt, q_ld, heads, cu_q, kv_len, rows, scale * 1.44269504f,
+                                 P.join ? P.sp.splits[0] : 1, C, qt, q_ld, heads, cu_q, kv_len, rows, scale_log2,
                                  P.sp.per[0], P.sp.splits[0], P.chunk ? 1 : 0, ot, out_ld, part))
       return why;
   }

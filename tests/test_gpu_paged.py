@@ -588,3 +588,21 @@ def test_attention_of_a_nan_key(pkg, lib, kind, d, kvh, news, lens, bad):
         assert bool(out[clear:].isnan().all()), (first, out[clear:].isnan().float().mean().item())
         if clear:
             check_attention(pool, q, heads, [clear], [kv - n + clear], out)
+
+
+@pytest.mark.parametrize("news", [[1, 2], [90, 3]])
+def test_attention_at_the_ends_of_the_scale(pkg, lib, news):
+    """The largest scales on equal scores, and a scale of zero on scores of 1e32: both are the mean."""
+    import torch
+    lens = [700, 150]
+    for scale, size in ((3.0e38, 0.0), (-3.0e38, 0.0), (0.0, 1e15)):
+        pool = Pool(pkg, torch.bfloat16, 2, 128, 32, lens, seed=33)
+        pool.fill(lens)
+        pg, sl = pool.where(0, torch.arange(700, device="cuda"))
+        pool.k[pg, sl] *= size
+        pg, sl = pool.where(1, torch.arange(150, device="cuda"))
+        pool.k[pg, sl] *= size
+        q = (torch.randn((sum(news), 8 * 128), device="cuda") * size).bfloat16()
+        out = torch.zeros_like(q)
+        attend(pkg, lib, pool, q, 8, news, lens, out, scale=scale)
+        check_attention(pool, q, 8, news, lens, out, scale=0.0)
