@@ -153,7 +153,6 @@ __device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, volati
       if (t0 == 0) t0 = t;
       if (t - t0 > W.ns) {
         *abort = 1u;
-        if (W.error) atomicCAS(W.error, 0u, kChunkError);
         return false;
       }
     }
@@ -828,6 +827,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   tc::tc_fence_before();
   __syncthreads();
   // a wait ran out: the rows of the item it ended, and of those that this CTA had taken on behind it, are NaN
+  if (s_abort && tid == 0 && W.error) atomicCAS(W.error, 0u, kChunkError);
   if (s_abort && warp < 8) {
     const int i = warp >> 2, total = count_items(C, cu_q, kv_len, rows, R, small_rows);
     for (int k = item; k < s_claims; ++k) {
