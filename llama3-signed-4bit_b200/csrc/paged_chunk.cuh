@@ -142,7 +142,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-// Waits (bounded) for phase `parity`; false after a timeout here or elsewhere in the CTA.
+// Waits (bounded) for phase `parity`; false after a timeout here or elsewhere in the CTA.  Every lane that
+// goes on to read what the phase guards polls for itself: what other threads and the asynchronous copies wrote
+// before it (an item, the answer of a takeover) is visible to those that saw it complete.  A lane that
+// polled for its warp and passed the outcome on by a shuffle, which orders no memory, would leave the others
+// with old items to make addresses from.
 __device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, const Waits& W) {
   unsigned long long t0 = 0;
   for (uint32_t n = 1;; ++n) {
@@ -410,7 +414,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       };
       auto stolen = [&] {  // the next item; -1: no more, or a wait ran out
         ok = wait(kSteal, steals - 1);
-        w = ok ? stolen_cta(smem_u32(s_steal)) : -1;
+        w = ok ? __shfl_sync(0xffffffffu, stolen_cta(smem_u32(s_steal)), 0) : -1;  // the warp's, as find_item wants it
         __syncwarp();
       };
       for (int k = 0; ok; ++k) {
