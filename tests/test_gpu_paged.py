@@ -606,3 +606,65 @@ def test_attention_at_the_ends_of_the_scale(pkg, lib, news):
         out = torch.zeros_like(q)
         attend(pkg, lib, pool, q, 8, news, lens, out, scale=scale)
         check_attention(pool, q, 8, news, lens, out, scale=0.0)
+
+
+FIRST_CALLS = """
+import ctypes, sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+from conftest import load_package
+pkg = load_package()
+from test_gpu_paged import Pool, rope
+lib = pkg.LlamaEngineBindings().lib
+news, lens, heads, kvh, d = [200, 1, 40, 1], [2600, 9000, 40, 700], 32, 8, 64
+rows, vocab = sum(news), 4099
+pool = Pool(pkg, torch.float16, kvh, d, 16, lens, seed=3)
+pool.fill(lens)
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+pos = i32(sum([list(range(n - m, n)) for m, n in zip(news, lens)], []))
+seq = i32(sum([[i] * m for i, m in enumerate(news)], []))
+cu, kvl = i32([0] + [sum(news[:i + 1]) for i in range(4)]), i32(lens)
+cos, sin = rope(d, 9000)
+qkv = torch.randn((rows, (heads + 2 * kvh) * d), device="cuda")
+lg, u = torch.randn((5, vocab), device="cuda"), torch.rand(5, device="cuda")
+k, p = i32([0, 5, 50, 0, 1]), torch.tensor([0.9, 1.0, 0.8, 1.0, 1.0], device="cuda")
+size = lib.llama_paged_attention_workspace(ctypes.byref(pool.desc), heads, rows, 200, 9000)
+ws = torch.empty((size + 16,), dtype=torch.uint8, device="cuda")
+q, out = [torch.zeros((rows, heads * d), dtype=torch.float16, device="cuda") for _ in range(2)]
+ids = torch.zeros(5, dtype=torch.int32, device="cuda")
+def calls(s):
+    rc = lib.llama_paged_append(ctypes.byref(pool.desc), qkv.data_ptr(), pkg.F32, qkv.stride(0), rows, heads, pos.data_ptr(),
+                                seq.data_ptr(), cos.data_ptr(), sin.data_ptr(), 9000, q.data_ptr(), pkg.F16, q.stride(0), s)
+    assert rc == 0, lib.llama_engine_last_error(None)
+    rc = lib.llama_paged_attention(ctypes.byref(pool.desc), q.data_ptr(), q.stride(0), heads, cu.data_ptr(), kvl.data_ptr(),
+                                   rows, 200, 9000, 0.125, out.data_ptr(), pkg.F16, out.stride(0), ws.data_ptr(), size, s)
+    assert rc == 0, lib.llama_engine_last_error(None)
+    rc = lib.llama_sample_rows(lg.data_ptr(), pkg.F32, vocab, 5, vocab, None, k.data_ptr(), p.data_ptr(), None, u.data_ptr(),
+                               ids.data_ptr(), s)
+    assert rc == 0, lib.llama_engine_last_error(None)
+torch.cuda.synchronize()
+side = torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    calls(side.cuda_stream)
+graph.replay()
+torch.cuda.synchronize()
+first = [x.clone() for x in (q, out, ids, pool.k.nan_to_num(9.0), pool.v.nan_to_num(9.0))]
+for x in (q, out, ids):
+    x.zero_()
+calls(0)
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(first, (q, out, ids, pool.k.nan_to_num(9.0), pool.v.nan_to_num(9.0))))
+assert bool((out != 0).any(dim=1).all())
+print("same")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured(pkg, gpu_available):
+    """Nothing has to run before a capture: the captured calls replay to the bits of later eager ones."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    code = FIRST_CALLS.format(root=str(ROOT), tests=str(ROOT / "tests"))
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.strip() == "same", res.stderr[-2000:]
