@@ -351,9 +351,9 @@ typedef struct llama_paged_kv {
  * llama_engine_rope_table makes them for head_dim 64), in fp32, rounded once.  type is LLAMA_F32 or
  * the cache's type; q_type is type or the cache's type.  A row with seq[t] outside [0, seqs) or
  * pos[t] outside [0, n_pos) is padding and writes nothing.  Of two rows with the same sequence and
- * position, either may be the one kept.  qkv, q_out and the tables are 16-byte aligned, ld and q_ld
- * multiples of 16 bytes.  Every pointer is memory of one device, which need not be the current one;
- * the call is queued on `stream` (a cudaStream_t of that device) and may be captured.  Returns 0, or
+ * position, either may be the one kept.  q_out overlaps neither qkv nor the pools.  qkv, q_out and the tables
+ * are 16-byte aligned, ld and q_ld multiples of 16 bytes.  Every pointer is memory of one device, which
+ * need not be the current one; the call is queued on `stream` (a cudaStream_t of that device) and may be captured.  Returns 0, or
  * -1 on bad arguments or a launch error (llama_engine_last_error(NULL) says which). */
 int llama_paged_append(const llama_paged_kv_t* kv, const void* qkv, int type, int64_t ld, int rows, int heads,
                        const int32_t* pos, const int32_t* seq, const float* rope_cos, const float* rope_sin,

@@ -110,7 +110,7 @@ __device__ __forceinline__ Span span_of(const Cache& C, const int32_t* cu_q, con
   const int a = cu_q[s], b = cu_q[s + 1];
   x.first = max(a, 0);
   x.n = min(b, rows) - x.first;
-  // a clipped sequence keeps its rows' positions: rows cut off at the end take keys with them
+  // clipping only keeps accesses in range: the callers' rows end at cu_q[seqs] <= rows
   x.len = max(0, min(kv_len[s], C.table_width << C.page_log2));
   return x;
 }
@@ -145,8 +145,8 @@ struct SplitPlan {
 // theirs.  D / 8 << groups_log2 threads per (row, head), 8 outputs each: a group of D / 8 takes every
 // groups-th split with a running (M, L, o), and the groups join through shared memory.  A thread's loads
 // follow one another's addresses only, so kCombineRun splits are in flight at a time.  Against one group
-// that walks all splits: attention of one token over 32768 keys (37 splits) 46 -> 18.5 us, over 4096
-// 23 -> 8.4 us.  Against looking every row of the call up: 32 chunks of 256 over 4096, with a single
+// that walks all splits: attention of one token, 8 kv heads of 64, over 32768 keys (64 splits) 26.5 -> 17.9
+// us, over 4096 (22) 10.7 -> 7.8 us.  Against looking every row of the call up: 32 chunks of 256 over 4096, with a single
 // token and an idle sequence among them, 279 -> 216 us.
 constexpr int kCombineThreads = 128, kCombineRun = 4;
 template <typename O, int D>

@@ -26,7 +26,8 @@
 //   * warps 0..3 and 4..7 are the softmax of tile 0 and 1, a thread per row (= tensor-memory lane), so
 //     that a row's maximum and sum need no exchange.  O is only rescaled when a row's maximum has
 //     grown by more than 2^8 since the value it is scaled by; until then weights may exceed 1, by at
-//     most 2^8, which costs no accuracy in fp32 sums or 16-bit weights.  A quarter of the
+//     most 2^8, which costs no accuracy in fp32 sums or 16-bit weights (this and the next are published
+//     techniques of tiled attention).  A quarter of the
 //     exponentials is computed on the FMA units (range reduction to
 //     |f| <= 1/2 and a polynomial of degree 5, 1e-7 relative), since 16 a clock and SM is what the
 //     special-function units give.
@@ -42,8 +43,11 @@
 // exponentials 770 on the special-function units and about 1,150 with the maxima, sums, conversions and
 // tensor-memory reads around them; two row tiles are under way at a time, and a key tile of both takes
 // 3,300 clocks with heads of 128.  One sequence of 8192 tokens, 32 heads: head_dim
-// 128 458 us (1201 TFLOP/s), 64 401 us (685).  8 x 2048, heads of 64: 247 us (557).  512 tokens over
-// 32768 keys, heads of 128: 251 us (1085).  Tried and no faster: 16 softmax warps, one pass over S held
+// 128 458 us (1201 TFLOP/s), 64 401 us (685).  512 tokens over 32768 keys, heads of 128: 251 us (1085) in a
+// burst, 283 to 295 us in a row of calls, under the power cap.  8 x 2048, heads of 64: 250 us (550), 3,900
+// clocks for a key tile of both row tiles, of which the arithmetic above explains 2,300: an item has 8.5 key
+// tiles here, its softmax warps themselves wait for its last product, read O and store it, and the diagonal
+// key tiles are computed whole.  Tried and no faster: 16 softmax warps, one pass over S held
 // in registers, a product warp for each row tile, other shares of polynomial exponentials (0, 3/8, 1/2).
 #pragma once
 

@@ -24,8 +24,8 @@
 // The weights are rounded to the cache's type for the product with v (the type its v has), the sum
 // l takes them unrounded in fp32.
 //
-// 128 sequences of up to 8192 keys, 8 kv heads of 128: 314 us, 2.07 GB at 6.6 TB/s, the rate of a plain
-// copy.  64 of up to 2048, heads of 64: 34.4 us (140 MB; 21 us at that rate): the rest is the launches, the
+// 128 sequences of up to 8192 keys, 8 kv heads of 128: 318 us, 2.07 GB at 6.5 TB/s, the rate of a plain
+// copy.  64 of up to 2048, heads of 64: 34.6 us (140 MB; 21 us at that rate): the rest is the launches, the
 // first loads (lengths, page, keys, one after the other), the last CTAs and the combine.  One sequence
 // of 700 keys: 6.1 us, all latency.
 #pragma once

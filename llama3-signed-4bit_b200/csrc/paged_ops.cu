@@ -202,8 +202,9 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   const int64_t units = (int64_t)std::min(kv->seqs, std::max(rows, 1)) * kv->kv_heads;
   // decode: a CTA's start and end cost as much as some hundred keys, and the last CTAs of many short ones
   // end closer together, so keys per CTA and CTAs grow alike, as the root of the call's keys.  At 0.9 of
-  // it (with a combine) 64 x 2048 takes 35.8 us (0.7 35.5, 1.4 37.6), 128 x 8192 333 us (332, 340), 1 x 4096
-  // 8.4 us (7.9, 9.9); 128 keys are two slices for each warp.
+  // it 64 x 2048 takes 34.6 us (0.7, with a quarter more parts in memory: 34.0; 1.4: 35.7), 128 x 8192 319
+  // us (313, 329), 1 x 4096 7.8 us (7.5, 9.0), 1 x 32768 17.9 us (17.5, 16.2); 128 keys are two slices for
+  // each warp.
   int64_t per = (int64_t)std::ceil(kKeysRoot * std::sqrt((double)units * keys));
   per = std::min(std::max<int64_t>(128, (per + 63) / 64 * 64), std::max<int64_t>(128, (keys + 63) / 64 * 64));
   int64_t parts = (keys + per - 1) / per;

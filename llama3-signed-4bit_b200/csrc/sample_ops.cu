@@ -22,12 +22,15 @@
 //     (key, index); the ids of the last bin are gathered.
 // No list is sorted: the border, or the draw, in a list is again found by a histogram (of counts or
 // masses, over bins in the list's order) and by comparing the few entries of one bin with each other.
-// What bounds it: the latency of those steps for few rows, the exponentials (64-bit) for many.  Device time
-// in us, all rows with the same rule:
+// What bounds it: the latency of those steps for few rows.  For many, that a row has an SM to itself, so that
+// its copy, its passes and their barriers follow one another (greedy rows, without a weight to compute, take
+// twice the copy's time), in two uneven waves of rows; then the weights (nine 64-bit operations and a look-up
+// in a table whose entries share banks) and, where the border lies far down, three atomics for each id.
+// Device time in us, all rows with the same rule:
 //                            greedy  T only  top_k 50  1000  top_p 0.9  0.95, T 1.2
-//   1 x 128256 fp32             4.1     9.8      13.3  17.4       17.0           38
-//   64 x 128256 fp32            9.5    25.5      29.1  37.0       43.2          105   (32.8 MB: 5.0 at the copy rate)
-//   256 x 50257 bf16           10.4    35.1      31.9  85.7       56.6          141   (25.7 MB: 3.9)
+//   1 x 128256 fp32             3.8     9.8      13.5  17.7       17.1           38
+//   64 x 128256 fp32            9.6    26.1      29.4  37.3       43.8          105   (32.8 MB: 5.0 at the copy rate)
+//   256 x 50257 bf16           10.4    35.5      32.1  86.2       56.7          141   (25.7 MB: 3.9)
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
