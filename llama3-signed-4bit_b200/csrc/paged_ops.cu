@@ -182,6 +182,7 @@ constexpr int kSms = 148;  // the workspace's size must not need a device
 constexpr int kSmSharedBytes = 227 * 1024;  // that an SM's CTAs can have together
 constexpr int kChunkItems = 4 * kSms;  // bounds what splitting makes
 constexpr double kKeysRoot = 0.9;
+constexpr int kIdleItems = 8192;  // decode CTAs of a call with more sequences than rows
 constexpr int kLongestBytes = 640 << 20;  // of keys and values when all have max_kv of them; L2 has 126 MB
 
 // How a call is cut: which kernels run, and their key splits.
@@ -205,9 +206,23 @@ static Plan plan_of(const llama_paged_kv_t* kv, int heads, int rows, int max_q, 
   // it 64 x 2048 takes 34.6 us (0.7, with a quarter more parts in memory: 34.0; 1.4: 35.7), 128 x 8192 319
   // us (313, 329), 1 x 4096 7.8 us (7.5, 9.0), 1 x 32768 17.9 us (17.5, 16.2); 128 keys are two slices for
   // each warp.
-  int64_t per = (int64_t)std::ceil(kKeysRoot * std::sqrt((double)units * keys));
-  per = std::min(std::max<int64_t>(128, (per + 63) / 64 * 64), std::max<int64_t>(128, (keys + 63) / 64 * 64));
+  auto whole = [](int64_t n) { return std::max<int64_t>(128, (n + 63) / 64 * 64); };
+  auto keys_each = [&](int64_t of) {
+    return std::min(whole((int64_t)std::ceil(kKeysRoot * std::sqrt((double)of * keys))), whole(keys));
+  };
+  int64_t per = keys_each(units);
   int64_t parts = (keys + per - 1) / per;
+  // Described sequences without a row launch as many CTAs and have room for as many parts as the others, so
+  // their number bounds the splits: one row over 8192 keys among 256 sequences (8 kv heads of 128) took 121 us
+  // and 570 MB for 32 splits, which it has alone.
+  const int64_t all = (int64_t)kv->seqs * kv->kv_heads;
+  if (all > units) {
+    const int64_t root = keys_each(all), most = std::max<int64_t>(kIdleItems / all, (keys + root - 1) / root);
+    if (parts > most) {
+      per = whole((keys + most - 1) / most);
+      parts = (keys + per - 1) / per;
+    }
+  }
   // Where all CTAs can be resident at once, a cluster of them takes each pair and joins its splits: no second
   // launch, no parts in memory, and every sequence cut evenly (1 x 700 9.2 -> 6.1 us, 16 x 2048 13.6 -> 12.7,
   // 8 x 2048 with heads of 128 19.0 -> 15.0).  Beyond that clusters wait for one another's shared memory (64 x

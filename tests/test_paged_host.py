@@ -107,3 +107,17 @@ def test_host_memory_is_refused(pkg, lib):
     assert attend(lib, kv) == -1
     assert sample(lib) == -1
     assert b"CUDA device" in lib.llama_engine_last_error(None)
+
+
+def test_workspace_of_sequences_without_rows(pkg, lib):
+    """Described sequences that may have no row bound the splits of those that have one: a single row among
+    many needs room for 8192 tiles and a split for each sequence, or as much as if all had rows."""
+    part = (128 + 8) * 4 * 16  # bytes of a decode tile's part, heads of 128
+    for keys in (2048, 8192, 32768):
+        for seqs in (1, 16, 64, 256, 1000):
+            kv = cache(pkg, num_pages=4096, page_size=64, kv_heads=8, head_dim=128, page_stride=64 * 1024, row_stride=1024,
+                       head_stride=128, table_stride=keys // 64, table_width=keys // 64, seqs=seqs)
+            size = lib.llama_paged_attention_workspace(ctypes.byref(kv), 32, 1, 1, keys)
+            # keys of a split grow as the root of the call's keys: at most the root's splits and one for each pair
+            full = (seqs * 8 * keys) ** 0.5 / 0.9 + seqs * 8
+            assert size <= max(8192 + seqs * 8, full) * part
